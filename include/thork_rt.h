@@ -322,6 +322,70 @@ THORK_API int thork_skinny_gemm_bf16_noalloc(const void *d_x, const void *d_w, v
  * counterpart.                                                             */
 THORK_API int thork_skinny_gemm_bf16_noalloc_status(unsigned *status, int clear, void *stream);
 
+/* ---- linear layers ------------------------------------------------------
+ * Matrix products with what surrounds them in a model's layers, and their
+ * gradients.  No reference counterpart (its tk.kernels.matmul is a plain
+ * product, src/thork/kernels/matmul.py:17-71).  All queue work on `stream`
+ * and return without synchronising; none allocates or keeps a workspace
+ * (the status word is allocated by the first call on a device, so make one
+ * call before a stream capture).  Arrays are dense row-major device memory,
+ * 16-byte aligned; bf16 unless said otherwise.  Sums are fp32; every output
+ * is rounded once.                                                         */
+enum {
+  THORK_ACT_NONE = 0,
+  THORK_ACT_RELU = 1,
+  THORK_ACT_GELU = 2,       /* z * Phi(z), Phi through erf                  */
+  THORK_ACT_GELU_TANH = 3,  /* 0.5 z (1 + tanh(sqrt(2/pi)(z + 0.044715 z^3))) */
+  THORK_ACT_SILU = 4        /* z / (1 + exp(-z))                            */
+};
+/* B is written by no kernel launched earlier on the stream (decode weights):
+ * products of few rows then start fetching it before the previous kernel
+ * has finished.  The others ignore the flag.                               */
+#define THORK_LINEAR_W_STATIC 1
+
+/* z = A[M,K] . B[K,N] + bias[N];  out = act(z) + residual[M,N].
+ * bias, residual and preact may be NULL; preact[M,N], when given, receives
+ * z, which the backward pass of an activation needs.  out may be the
+ * residual itself; otherwise outputs may not overlap inputs or one another.
+ * K and N multiples of 8.                                                  */
+THORK_API int thork_linear_bf16(const void *d_a, const void *d_b, void *d_out, const void *d_bias,
+                                const void *d_residual, void *d_preact, int M, int N, int K,
+                                int activation, int flags, void *stream);
+/* The same with A and B float8 e4m3: z = scale_a * scale_b * (A . B) + bias.
+ * K and N multiples of 16.                                                 */
+THORK_API int thork_linear_e4m3(const void *d_a, const void *d_b, void *d_out, const void *d_bias,
+                                const void *d_residual, void *d_preact, int M, int N, int K,
+                                float scale_a, float scale_b, int activation, int flags, void *stream);
+/* Gradients of thork_linear_bf16 from dout[M,N] (which is the residual's own
+ * gradient): dpre = dout * act'(preact), dbias[N] (fp32) = column sums of
+ * dpre before its rounding, dA[M,K] = dpre . B^T, dB[K,N] = A^T . dpre.
+ * Each of dA, dB, dbias may be NULL and is then not computed.  preact and
+ * dpre are required with an activation and NULL without one (dpre is dout
+ * then).  The bf16 rounding of dpre is what the tensor cores read.         */
+THORK_API int thork_linear_backward_bf16(void *d_da, void *d_db, float *d_dbias, const void *d_dout,
+                                         const void *d_a, const void *d_b, const void *d_preact,
+                                         void *d_dpre, int M, int N, int K, int activation, void *stream);
+/* Products grouped by expert: rows [offsets[e], offsets[e+1]) of A[T,K] times
+ * B[e] of B[E,K,N], into the same rows of out[T,N], through an activation
+ * when asked.  offsets[E+1] (int32, device) are non-decreasing within
+ * [0, T]; groups may be empty, and rows outside every group are left as they
+ * were in every output.  Offsets that are not are clamped into the buffer
+ * (no access leaves it) and recorded in the status word.  E <= 1024.       */
+THORK_API int thork_grouped_gemm_bf16(const void *d_a, const void *d_b, void *d_out, const int *d_offsets,
+                                      void *d_preact, int E, int T, int N, int K, int activation,
+                                      int flags, void *stream);
+/* The same with e4m3 A and B: z = scale_a * scale_b[e] * (A . B[e]);
+ * d_scale_b[E] is fp32 device memory, NULL for all ones.                   */
+THORK_API int thork_grouped_gemm_e4m3(const void *d_a, const void *d_b, void *d_out, const int *d_offsets,
+                                      void *d_preact, int E, int T, int N, int K, float scale_a,
+                                      const float *d_scale_b, int activation, int flags, void *stream);
+/* Gradients of thork_grouped_gemm_bf16: as thork_linear_backward_bf16 on
+ * each group's rows, dB[E,K,N] per group (zeros for an empty one).         */
+THORK_API int thork_grouped_gemm_backward_bf16(void *d_da, void *d_db, const void *d_dout, const void *d_a,
+                                               const void *d_b, const int *d_offsets, const void *d_preact,
+                                               void *d_dpre, int E, int T, int N, int K, int activation,
+                                               void *stream);
+
 /* ---- NVLink multicast buffers (no reference counterpart) ---------------
  * For the fused GEMM + all-gather over NVSwitch multicast ("NVLS"): every
  * GPU of a group binds memory of its own to one multicast object, and a

@@ -1,0 +1,201 @@
+"""GPU: tk.kernels.grouped_matmul and its backward pass against their 64-bit
+forms, group by group (tolerances derived in linear_ref.py)."""
+
+import numpy as np
+import pytest
+
+import thork_b200 as tk
+from linear_ref import act, act_err, bits, close, product, sizes_to_offsets, slope, slope_err, wide
+from oracle import oracle
+
+pytestmark = pytest.mark.gpu
+rt = tk.runtime
+
+# sizes per expert, first row, rows of the buffer behind the last group
+GROUPS = {
+    "one": ([5], 0, 0),
+    "empty": ([0, 0, 0], 0, 4),
+    "single rows": ([1, 0, 1, 1], 0, 0),
+    "thin": ([0, 3, 16, 17, 0, 1, 40, 2], 0, 5),
+    "first offset": ([7, 0, 9], 6, 3),
+    "tiles": ([64, 65, 128, 127, 63, 1], 0, 0),
+    "wide": ([300, 0, 257, 256, 513], 0, 11),
+    "skewed": ([1000, 2, 0, 130], 1, 1),
+    "many": ([(i * 7) % 23 for i in range(70)], 0, 9),
+}
+
+
+@pytest.fixture(autouse=True)
+def _status():
+    yield
+    assert rt.kernel_status() == 0
+
+
+def _layout(name):
+    sizes, first, behind = GROUPS[name]
+    off = sizes_to_offsets(sizes, first)
+    return off, int(off[-1]) + behind
+
+
+def _inside(off, t):
+    return (np.arange(t) >= off[0]) & (np.arange(t) < off[-1])
+
+
+@pytest.mark.parametrize("n,k", [(136, 72), (264, 1032)])
+@pytest.mark.parametrize("name", sorted(GROUPS))
+def test_grouped_matmul(name, n, k):
+    off, t = _layout(name)
+    e = len(off) - 1
+    rng = np.random.default_rng(1)
+    a, b = bits(rng, t, k), bits(rng, e, k, n, std=1.2 / np.sqrt(k))
+    a[~_inside(off, t)] = 0x7FC0  # NaN in rows of no group must not spread
+    for activation, keep in (("none", False), ("silu", True)):
+        out = bits(rng, t, n)
+        pre = bits(rng, t, n) if keep else None
+        before, before_pre = out.copy(), None if pre is None else pre.copy()
+        tk.kernels.grouped_matmul(e, t, n, k, activation=activation)(out, a, b, off, preact=pre)
+        for i in range(e):
+            r = slice(off[i], off[i + 1])
+            z, err = product(wide(a[r]), wide(b[i]))
+            if keep:
+                close(pre[r], z, err, f"preact of group {i}") if z.size else None
+            if z.size:
+                close(out[r], act(z, activation), act_err(z, err), f"group {i}")
+        rest = ~_inside(off, t)
+        np.testing.assert_array_equal(out[rest], before[rest])
+        if keep:
+            np.testing.assert_array_equal(pre[rest], before_pre[rest])
+
+
+@pytest.mark.parametrize("name", ["thin", "wide", "many", "tiles"])
+@pytest.mark.parametrize("scaled", [True, False])
+def test_grouped_matmul_e4m3(name, scaled):
+    off, t = _layout(name)
+    e, n, k = len(off) - 1, 272, 208
+    rng = np.random.default_rng(2)
+    qa, sa = tk.dt.quantize_e4m3(rng.standard_normal((t, k), dtype=np.float32))
+    qb = np.stack([tk.dt.quantize_e4m3(rng.standard_normal((k, n), dtype=np.float32))[0] for _ in range(e)])
+    sb = (0.5 + rng.random(e)).astype(np.float32) / 1000 if scaled else None
+    out = bits(rng, t, n)
+    before = out.copy()
+    tk.kernels.grouped_matmul(e, t, n, k, tk.dt.float8_e4m3, activation="gelu_tanh")(
+        out, qa, qb, off, scale_a=sa, scale_b=sb)
+    A, B = oracle.e4m3_bits_to_f32(qa).astype(np.float64), oracle.e4m3_bits_to_f32(qb).astype(np.float64)
+    for i in range(e):
+        r = slice(off[i], off[i + 1])
+        s = sa * (float(sb[i]) if scaled else 1.0)
+        z, err = product(A[r], B[i])
+        z, err = z * s, err * s + 2.0 ** -22 * np.abs(z) * s
+        if z.size:
+            close(out[r], act(z, "gelu_tanh"), act_err(z, err), f"group {i}")
+    rest = ~_inside(off, t)
+    np.testing.assert_array_equal(out[rest], before[rest])
+
+
+@pytest.mark.parametrize("n,k", [(136, 72), (520, 264)])
+@pytest.mark.parametrize("name", sorted(GROUPS))
+def test_grouped_backward(name, n, k):
+    off, t = _layout(name)
+    e = len(off) - 1
+    rng = np.random.default_rng(3)
+    a, b = bits(rng, t, k), bits(rng, e, k, n, std=1.2 / np.sqrt(k))
+    dout, z = bits(rng, t, n, std=1 / 64), bits(rng, t, n, std=1.5)
+    rest = ~_inside(off, t)
+    a[rest] = dout[rest] = z[rest] = 0x7FC0  # NaN behind the groups must not enter a sum
+    for activation in ("none", "gelu_tanh"):
+        bent = activation != "none"
+        da, dz = bits(rng, t, k), bits(rng, t, n) if bent else None
+        # dz of the rows of no group keeps NaN too: the weight gradient's last
+        # rows of a group are loaded together with it
+        if bent:
+            dz[rest] = 0x7FC0
+        before, before_dz = da.copy(), dz.copy() if bent else None
+        db = np.full((e, k, n), 0x7FC0, np.uint16)
+        tk.kernels.grouped_matmul_backward(e, t, n, k, activation=activation)(
+            da, db, dout, a, b, off, z if bent else None, dz)
+        for i in range(e):
+            r = slice(off[i], off[i + 1])
+            g = wide(dout[r])
+            if bent and g.size:
+                want = g * slope(wide(z[r]), activation)
+                close(dz[r], want, np.abs(g) * slope_err(wide(z[r])), f"dpre of group {i}")
+            gz = wide(dz[r]) if bent else g
+            if g.size:
+                close(da[r], *product(gz, wide(b[i]).T), f"dA of group {i}")
+                close(db[i], *product(wide(a[r]).T, gz), f"dB of group {i}")
+            else:
+                assert (db[i] == 0).all(), f"dB of the empty group {i}"
+        np.testing.assert_array_equal(da[rest], before[rest])
+        if bent:
+            np.testing.assert_array_equal(dz[rest], before_dz[rest])
+
+
+def test_group_with_nan_leaves_the_others_gradients_alone():
+    """The last k-block of a group's weight gradient also loads the next
+    group's first rows: a NaN there must not count."""
+    off = sizes_to_offsets([70, 40, 3])
+    e, t, n, k = 3, 113, 136, 136
+    rng = np.random.default_rng(4)
+    a, b, dout = bits(rng, t, k), bits(rng, e, k, n), bits(rng, t, n)
+    f = tk.kernels.grouped_matmul_backward(e, t, n, k)
+    clean = np.zeros((e, k, n), np.uint16)
+    f(None, clean, dout, a, None, off)
+    a[70:110] = 0x7FC0
+    dout[70:110] = 0xFF80
+    got = np.zeros((e, k, n), np.uint16)
+    f(None, got, dout, a, None, off)
+    np.testing.assert_array_equal(got[[0, 2]], clean[[0, 2]])
+    assert np.isnan(oracle.bf16_bits_to_f32(got[1])).all()
+
+
+def test_offsets_that_are_wrong_are_clamped_and_reported():
+    e, t, n, k = 4, 40, 136, 72
+    rng = np.random.default_rng(5)
+    a, b = bits(rng, t, k), bits(rng, e, k, n)
+    off = np.array([-5, 10, 7, 1000, 20], np.int32)  # reads as 0, 10, 10, 40, 40
+    want = np.zeros((t, n), np.uint16)
+    f = tk.kernels.grouped_matmul(e, t, n, k)
+    f(want, a, b, np.array([0, 10, 10, 40, 40], np.int32))
+    assert rt.kernel_status() == 0
+    out = np.zeros((t, n), np.uint16)
+    f(out, a, b, off)
+    assert rt.kernel_status() & 0xFF == 2
+    np.testing.assert_array_equal(out, want)
+
+
+def test_expert_layers_forward_and_backward():
+    """Two grouped layers with an activation between, forward and backward,
+    asynchronously on one stream, with offsets that live on the device."""
+    sizes = [30, 0, 100, 7, 260]
+    off = sizes_to_offsets(sizes)
+    e, t, d, f = len(sizes), int(off[-1]), 136, 264
+    rng = np.random.default_rng(6)
+    x, w1, w2 = bits(rng, t, d), bits(rng, e, d, f, std=0.1), bits(rng, e, f, d, std=0.06)
+    dy = bits(rng, t, d, std=0.1)
+    D = {n: rt.to_device(v) for n, v in dict(x=x, w1=w1, w2=w2, dy=dy, off=off).items()}
+    h, z, dz, dh = (rt.empty((t, f), np.uint16) for _ in range(4))
+    y, dx = rt.empty((t, d), np.uint16), rt.empty((t, d), np.uint16)
+    dw1, dw2 = rt.empty((e, d, f), np.uint16), rt.empty((e, f, d), np.uint16)
+    s = rt.Stream()
+    kw = dict(stream=s, sync=False)
+    K = tk.kernels
+    K.grouped_matmul(e, t, f, d, activation="silu")(h, D["x"], D["w1"], D["off"], preact=z, **kw)
+    K.grouped_matmul(e, t, d, f)(y, h, D["w2"], D["off"], **kw)
+    K.grouped_matmul_backward(e, t, d, f)(dh, dw2, D["dy"], h, D["w2"], D["off"], **kw)
+    K.grouped_matmul_backward(e, t, f, d, activation="silu")(dx, dw1, dh, D["x"], D["w1"], D["off"], z, dz, **kw)
+    s.synchronize()
+    for i in range(e):
+        r = slice(off[i], off[i + 1])
+        if sizes[i] == 0:
+            assert (dw1.to_host()[i] == 0).all() and (dw2.to_host()[i] == 0).all()
+            continue
+        H, DH, DZ = (wide(v.to_host()[r]) for v in (h, dh, dz))
+        zz, err = product(wide(x[r]), wide(w1[i]))
+        close(h.to_host()[r], act(zz, "silu"), act_err(zz, err), "h")
+        close(y.to_host()[r], *product(H, wide(w2[i])), "y")
+        close(dh.to_host()[r], *product(wide(dy[r]), wide(w2[i]).T), "dh")
+        close(dw2.to_host()[i], *product(H.T, wide(dy[r])), "dw2")
+        zb = wide(z.to_host()[r])
+        close(dz.to_host()[r], DH * slope(zb, "silu"), np.abs(DH) * slope_err(zb), "dz")
+        close(dx.to_host()[r], *product(DZ, wide(w1[i]).T), "dx")
+        close(dw1.to_host()[i], *product(wide(x[r]).T, DZ), "dw1")

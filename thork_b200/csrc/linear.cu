@@ -1,0 +1,409 @@
+// linear.cu — the linear-layer operators of libthork_rt.so and their C-ABI
+// entry points (declared in include/thork_rt.h):
+//   thork_linear_{bf16,e4m3}             product + bias + activation + residual
+//   thork_linear_backward_bf16           its gradients
+//   thork_grouped_gemm_{bf16,e4m3}       products grouped by expert, ragged sizes
+//   thork_grouped_gemm_backward_bf16     their gradients
+// Kernels: device/linear_sm100.cuh.  No call allocates memory or keeps a
+// workspace, so calls on different streams, and graphs that captured them,
+// share nothing but the status word.
+#include <cuda_runtime.h>
+
+#include <atomic>
+#include <cstdint>
+
+#include "device/linear_sm100.cuh"
+#include "thork_internal.h"
+#include "thork_rt.h"
+
+using thork::dev::TensorMap;
+
+namespace {
+using namespace thork::lin;
+
+// ---------------------------------------------------------------- launching
+// Opt in to a kernel's dynamic shared memory, once per kernel and device.
+int allow_smem(const void *kernel, int bytes, std::atomic<uint64_t> &done) {
+  int dev;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return thork_cuda_error(e, "cudaGetDevice");
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_acquire) & bit) return THORK_OK;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return thork_cuda_error(e, "cudaFuncSetAttribute(max dynamic smem)");
+  done.fetch_or(bit, std::memory_order_release);
+  return THORK_OK;
+}
+
+// Launch in clusters of `cluster` CTAs, with programmatic stream
+// serialisation: the kernels wait for the previous one before they touch
+// memory that it may write.
+template <class... KArgs, class... Args>
+int launch(void (*kern)(KArgs...), unsigned grid, int threads, int smem, int cluster, cudaStream_t s,
+           const char *what, const Args &...args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid, 1, 1);
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+  return e == cudaSuccess ? THORK_OK : thork_cuda_error(e, what);
+}
+
+template <class C>
+int run_pair(const TensorMap &ta, const TensorMap &tb, const GemmArgs &g, long long tiles,
+             cudaStream_t s, const char *what) {
+  static std::atomic<uint64_t> done{0};
+  int rc, sms;
+  auto kern = pair_kernel<C>;
+  if ((rc = allow_smem(reinterpret_cast<const void *>(kern), C::SMEM_BYTES, done))) return rc;
+  if ((rc = thork_sm_count(&sms))) return rc;
+  const int pairs = static_cast<int>(tiles < sms / 2 ? tiles : sms / 2);
+  return launch(kern, 2 * pairs, C::THREADS, C::SMEM_BYTES, 2, s, what, ta, tb, g);
+}
+
+template <class C>
+int run_swap(const TensorMap &tw, const TensorMap &tx, const GemmArgs &g, long long items, int split,
+             cudaStream_t s, const char *what) {
+  static std::atomic<uint64_t> done{0};
+  int rc;
+  auto kern = swap_kernel<C>;
+  if ((rc = allow_smem(reinterpret_cast<const void *>(kern), C::SMEM_BYTES, done))) return rc;
+  if (items * split > 0x7fffffffll)
+    return thork_set_error(THORK_ERR_INVALID, "%s: %lld tiles are more than a launch can hold", what, items);
+  return launch(kern, static_cast<unsigned>(items * split), C::THREADS, C::SMEM_BYTES, split, s, what, tw,
+                tx, g);
+}
+
+// ---------------------------------------------------------------- a product
+// One (grouped) product in GEMM terms: out[m, n] = sum_k X[m, k] W[k, n], X
+// row-major [rows, k], W either as stored ([k, n] row-major, W_MN) or its
+// transpose ([n, k] row-major).
+struct Product {
+  const void *x, *w;
+  int rows, n, k;  // rows of X (of the buffer when grouped)
+  int groups;      // 0: dense
+};
+
+// k-blocks per CTA below which splitting the contraction further costs more
+// (one more partial tile to sum) than its shorter loop saves
+constexpr int kMinSplitBlocks = 4;
+
+template <int KIND, bool W_MN>
+int map_w(TensorMap &t, const Product &p, int box_n) {
+  const int elem = KIND == KIND_BF16 ? 2 : 1;
+  const int dt = KIND == KIND_BF16 ? THORK_DT_BF16 : THORK_DT_E4M3;
+  const uint64_t e = p.groups ? p.groups : 1;
+  if (W_MN)
+    return thork_encode_tmap_3d(&t, dt, p.w, p.n, p.k, e, 128 / elem, 128 / elem);
+  return thork_encode_tmap_3d(&t, dt, p.w, p.k, p.n, e, 128 / elem, box_n);
+}
+
+template <int KIND>
+int map_x(TensorMap &t, const Product &p, int box_rows) {
+  const int elem = KIND == KIND_BF16 ? 2 : 1;
+  return thork_encode_tmap_3d(&t, KIND == KIND_BF16 ? THORK_DT_BF16 : THORK_DT_E4M3, p.x, p.k, p.rows, 1,
+                              128 / elem, box_rows);
+}
+
+template <int KIND, int BN, int STAGES, bool W_MN, bool GROUPED>
+int swap_product(const Product &p, const GemmArgs &g, cudaStream_t s, const char *what) {
+  using C = SwapCfg<KIND, BN, STAGES, W_MN, GROUPED>;
+  int rc, sms;
+  alignas(64) TensorMap tw, tx;
+  if ((rc = map_w<KIND, W_MN>(tw, p, C::BM))) return rc;
+  if ((rc = map_x<KIND>(tx, p, BN))) return rc;
+  if ((rc = thork_sm_count(&sms))) return rc;
+  const long long ntn = (p.n + C::BM - 1) / C::BM;
+  long long rt = (p.rows + BN - 1) / BN, likely = rt;
+  if (GROUPED) {
+    // at most one partial tile per group that has rows
+    const long long most = (static_cast<long long>(p.rows) + static_cast<long long>(p.groups) * (BN - 1)) / BN;
+    rt = most < p.rows ? most : p.rows;
+    const long long held = p.groups < p.rows ? p.groups : p.rows;
+    likely = likely > held ? likely : held;
+  }
+  // two CTAs fit on an SM: split the contraction until they are all in use
+  const int nkb = (p.k + C::BK - 1) / C::BK;
+  long long split = 2ll * sms / (likely * ntn);
+  if (split > nkb / kMinSplitBlocks) split = nkb / kMinSplitBlocks;
+  if (split > 8) split = 8;
+  if (split < 1) split = 1;
+  return run_swap<C>(tw, tx, g, rt * ntn, static_cast<int>(split), s, what);
+}
+
+template <int KIND, int BN, int STAGES, bool W_MN, int MODE>
+int pair_product(const Product &p, const GemmArgs &g, cudaStream_t s, const char *what) {
+  using C = PairCfg<KIND, BN, STAGES, false, W_MN, MODE>;
+  int rc;
+  alignas(64) TensorMap ta, tb;
+  if ((rc = map_x<KIND>(ta, p, C::BM))) return rc;
+  if ((rc = map_w<KIND, W_MN>(tb, p, C::BNH))) return rc;
+  long long rt = (p.rows + 255) / 256;
+  if (MODE == GROUP_ROWS) rt += p.groups < p.rows ? p.groups : p.rows;
+  return run_pair<C>(ta, tb, g, rt * ((p.n + BN - 1) / BN), s, what);
+}
+
+template <int KIND, bool W_MN, bool GROUPED>
+int product(const Product &p, const GemmArgs &g, cudaStream_t s, const char *what) {
+  constexpr int MODE = GROUPED ? GROUP_ROWS : DENSE;
+  int rc, sms;
+  if ((rc = thork_sm_count(&sms))) return rc;
+  // rows that a tile can expect: of the whole product, or of one group
+  const long long rows = GROUPED ? (static_cast<long long>(p.rows) + p.groups - 1) / p.groups : p.rows;
+  constexpr int G = GROUPED ? 1 : 0;  // the group table takes one stage's room
+  if (rows <= 16) return swap_product<KIND, 16, 6 - G, W_MN, GROUPED>(p, g, s, what);
+  if (rows <= 32) return swap_product<KIND, 32, 5, W_MN, GROUPED>(p, g, s, what);
+  if (rows <= 64) return swap_product<KIND, 64, 4, W_MN, GROUPED>(p, g, s, what);
+  if (rows <= 128) return swap_product<KIND, 128, 3, W_MN, GROUPED>(p, g, s, what);
+  if constexpr (KIND == KIND_BF16) {
+    const long long tiles = ((p.rows + 255) / 256) * static_cast<long long>((p.n + 255) / 256);
+    if (tiles < sms / 2) return pair_product<KIND, 128, 8 - 2 * G, W_MN, MODE>(p, g, s, what);
+  }
+  return pair_product<KIND, 256, 6 - G, W_MN, MODE>(p, g, s, what);
+}
+
+// dW[k, n] = sum over rows X[m, k] dY[m, n], of each group's rows when grouped.
+template <int BN, int STAGES, int MODE>
+int weight_gradient(const void *x, const void *dy, int rows, int n, int k, int groups, const GemmArgs &g,
+                    cudaStream_t s, const char *what) {
+  using C = PairCfg<KIND_BF16, BN, STAGES, true, true, MODE>;
+  int rc;
+  alignas(64) TensorMap ta, tb;
+  if ((rc = thork_encode_tmap_3d(&ta, THORK_DT_BF16, x, k, rows, 1, 64, 64))) return rc;
+  if ((rc = thork_encode_tmap_3d(&tb, THORK_DT_BF16, dy, n, rows, 1, 64, 64))) return rc;
+  const long long tiles = ((k + 255) / 256) * static_cast<long long>((n + BN - 1) / BN) * (groups ? groups : 1);
+  return run_pair<C>(ta, tb, g, tiles, s, what);
+}
+
+int slope(const SlopeArgs &a, cudaStream_t s, const char *what) {
+  int rc, sms;
+  if ((rc = thork_sm_count(&sms))) return rc;
+  const long long stripes = (a.cols + 127) / 128;
+  // eight blocks of 256 threads per SM, at most one per 64 rows
+  long long split = 8ll * sms / stripes;
+  const long long most = (a.rows + 63) / 64;
+  if (split > most) split = most;
+  if (split > 8) split = 8;
+  if (split < 1) split = 1;
+  return launch(slope_kernel, static_cast<unsigned>(stripes * split), 256, 0, static_cast<int>(split), s,
+                what, a);
+}
+
+// ---------------------------------------------------------------- checks
+int check_sizes(int rows, int n, int k, int align, const char *what) {
+  if (rows <= 0 || n <= 0 || k <= 0)
+    return thork_set_error(THORK_ERR_INVALID, "%s: dimensions must be positive (M=%d N=%d K=%d)", what,
+                           rows, n, k);
+  if (n % align || k % align)
+    return thork_set_error(THORK_ERR_INVALID,
+                           "%s: K and N must be multiples of %d for 16-byte TMA row strides (M=%d N=%d K=%d)",
+                           what, align, rows, n, k);
+  return THORK_OK;
+}
+
+int check_groups(int groups, const void *offsets, const char *what) {
+  if (groups < 1 || groups > kMaxGroups)
+    return thork_set_error(THORK_ERR_INVALID, "%s: E=%d must be 1..%d", what, groups, kMaxGroups);
+  if (!offsets || (reinterpret_cast<uintptr_t>(offsets) & 3u))
+    return thork_set_error(THORK_ERR_INVALID, "%s: offsets are NULL or not 4-byte aligned", what);
+  return THORK_OK;
+}
+
+int check_act(int act, const char *what) {
+  if (act < THORK_ACT_NONE || act > THORK_ACT_SILU)
+    return thork_set_error(THORK_ERR_INVALID, "%s: unknown activation %d", what, act);
+  return THORK_OK;
+}
+
+// One array argument: required ones may not be NULL, all are 16-byte aligned.
+struct Arg {
+  const void *p;
+  const char *name;
+  bool required, output;
+};
+
+template <size_t N>
+int check_args(const Arg (&args)[N], const char *what) {
+  for (const Arg &a : args) {
+    if (a.required && !a.p) return thork_set_error(THORK_ERR_INVALID, "%s: %s is NULL", what, a.name);
+    if (reinterpret_cast<uintptr_t>(a.p) & 15u)
+      return thork_set_error(THORK_ERR_INVALID, "%s: %s must be 16-byte aligned", what, a.name);
+  }
+  for (const Arg &o : args)
+    for (const Arg &i : args)
+      if (o.output && o.p && o.p == i.p && &o != &i)
+        return thork_set_error(THORK_ERR_INVALID, "%s: %s and %s are the same array", what, o.name, i.name);
+  return THORK_OK;
+}
+
+template <int KIND>
+int linear(const void *a, const void *b, void *c, const void *bias, const void *residual, void *preact,
+           int M, int N, int K, float alpha, int act, int flags, void *stream, const char *what) {
+  int rc;
+  if ((rc = check_sizes(M, N, K, KIND == KIND_BF16 ? 8 : 16, what))) return rc;
+  if ((rc = check_act(act, what))) return rc;
+  if (flags & ~THORK_LINEAR_W_STATIC)
+    return thork_set_error(THORK_ERR_INVALID, "%s: unknown flags 0x%x", what, flags);
+  const Arg args[] = {{a, "A", true, false}, {b, "B", true, false}, {bias, "bias", false, false},
+                      {c, "out", true, true}, {preact, "preact", false, true}};
+  if ((rc = check_args(args, what))) return rc;
+  const Arg inplace[] = {{residual, "residual", false, false}, {preact, "preact", false, true}};
+  if ((rc = check_args(inplace, what))) return rc;  // out may be the residual itself
+  GemmArgs g = {};
+  g.epi = {static_cast<unsigned short *>(c), static_cast<unsigned short *>(preact),
+           static_cast<const unsigned short *>(bias), static_cast<const unsigned short *>(residual),
+           nullptr, alpha, act, N, nullptr};
+  if ((rc = thork_status_word(&g.epi.status))) return rc;
+  g.GM = g.rows = M;
+  g.GN = N;
+  g.GK = K;
+  g.w_static = flags & THORK_LINEAR_W_STATIC;
+  return product<KIND, true, false>({a, b, M, N, K, 0}, g, static_cast<cudaStream_t>(stream), what);
+}
+
+template <int KIND>
+int grouped(const void *a, const void *b, void *c, const int *offsets, void *preact, int E, int T, int N,
+            int K, float alpha, const float *group_scale, int act, int flags, void *stream,
+            const char *what) {
+  int rc;
+  if ((rc = check_sizes(T, N, K, KIND == KIND_BF16 ? 8 : 16, what))) return rc;
+  if ((rc = check_groups(E, offsets, what))) return rc;
+  if ((rc = check_act(act, what))) return rc;
+  if (flags & ~THORK_LINEAR_W_STATIC)
+    return thork_set_error(THORK_ERR_INVALID, "%s: unknown flags 0x%x", what, flags);
+  const Arg args[] = {{a, "A", true, false}, {b, "B", true, false}, {c, "out", true, true},
+                      {preact, "preact", false, true}};
+  if ((rc = check_args(args, what))) return rc;
+  if (reinterpret_cast<uintptr_t>(group_scale) & 3u)
+    return thork_set_error(THORK_ERR_INVALID, "%s: scale_b is not 4-byte aligned", what);
+  GemmArgs g = {};
+  g.epi = {static_cast<unsigned short *>(c), static_cast<unsigned short *>(preact), nullptr, nullptr,
+           group_scale, alpha, act, N, nullptr};
+  if ((rc = thork_status_word(&g.epi.status))) return rc;
+  g.GM = g.rows = T;
+  g.GN = N;
+  g.GK = K;
+  g.offsets = offsets;
+  g.groups = E;
+  return product<KIND, true, true>({a, b, T, N, K, E}, g, static_cast<cudaStream_t>(stream), what);
+}
+
+// Gradients of a (grouped) linear layer from dout and, with an activation,
+// the pre-activation; groups == 0 is the dense layer.
+int backward(void *da, void *db, float *dbias, const void *dout, const void *a, const void *b,
+             const void *preact, void *dpre, const int *offsets, int groups, int rows, int N, int K,
+             int act, void *stream, const char *what) {
+  int rc;
+  if ((rc = check_sizes(rows, N, K, 8, what))) return rc;
+  if ((rc = check_act(act, what))) return rc;
+  const bool bent = act != THORK_ACT_NONE;
+  if (bent != (preact != nullptr) || bent != (dpre != nullptr))
+    return thork_set_error(THORK_ERR_INVALID,
+                           "%s: preact and dpre go with an activation, and with one only", what);
+  const Arg args[] = {{dout, "dout", true, false}, {a, "A", db != nullptr, false},
+                      {b, "B", da != nullptr, false}, {preact, "preact", false, false},
+                      {dpre, "dpre", false, true}, {da, "dA", false, true}, {db, "dB", false, true},
+                      {dbias, "dbias", false, true}};
+  if ((rc = check_args(args, what))) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (bent || dbias) {
+    const SlopeArgs sl = {static_cast<const unsigned short *>(dout),
+                          static_cast<const unsigned short *>(preact), static_cast<unsigned short *>(dpre),
+                          dbias, rows, N, act, offsets, groups};
+    if ((rc = slope(sl, s, what))) return rc;
+  }
+  const void *dz = bent ? dpre : dout;
+  GemmArgs g = {};
+  g.epi.alpha = 1.0f;
+  if ((rc = thork_status_word(&g.epi.status))) return rc;
+  g.rows = rows;
+  g.offsets = offsets;
+  g.groups = groups;
+  if (da) {
+    GemmArgs d = g;
+    d.epi.out = static_cast<unsigned short *>(da);
+    d.epi.cols = K;
+    d.GM = rows;
+    d.GN = K;
+    d.GK = N;
+    const Product p = {dz, b, rows, K, N, groups};
+    rc = groups ? product<KIND_BF16, false, true>(p, d, s, what) : product<KIND_BF16, false, false>(p, d, s, what);
+    if (rc) return rc;
+  }
+  if (db) {
+    int sms;
+    if ((rc = thork_sm_count(&sms))) return rc;
+    GemmArgs w = g;
+    w.epi.out = static_cast<unsigned short *>(db);
+    w.epi.cols = N;
+    w.GM = K;
+    w.GN = N;
+    w.GK = rows;
+    const long long tiles = ((K + 255) / 256) * static_cast<long long>((N + 255) / 256) * (groups ? groups : 1);
+    const bool wide = tiles >= sms / 2;
+    if (groups)
+      rc = wide ? weight_gradient<256, 5, GROUP_K>(a, dz, rows, N, K, groups, w, s, what)
+                : weight_gradient<128, 6, GROUP_K>(a, dz, rows, N, K, groups, w, s, what);
+    else
+      rc = wide ? weight_gradient<256, 6, DENSE>(a, dz, rows, N, K, 0, w, s, what)
+                : weight_gradient<128, 8, DENSE>(a, dz, rows, N, K, 0, w, s, what);
+    if (rc) return rc;
+  }
+  return THORK_OK;
+}
+}  // namespace
+
+extern "C" int thork_linear_bf16(const void *d_a, const void *d_b, void *d_out, const void *d_bias,
+                                 const void *d_residual, void *d_preact, int M, int N, int K,
+                                 int activation, int flags, void *stream) {
+  return linear<KIND_BF16>(d_a, d_b, d_out, d_bias, d_residual, d_preact, M, N, K, 1.0f, activation, flags,
+                           stream, "linear_bf16");
+}
+
+extern "C" int thork_linear_e4m3(const void *d_a, const void *d_b, void *d_out, const void *d_bias,
+                                 const void *d_residual, void *d_preact, int M, int N, int K,
+                                 float scale_a, float scale_b, int activation, int flags, void *stream) {
+  return linear<KIND_E4M3>(d_a, d_b, d_out, d_bias, d_residual, d_preact, M, N, K, scale_a * scale_b,
+                           activation, flags, stream, "linear_e4m3");
+}
+
+extern "C" int thork_linear_backward_bf16(void *d_da, void *d_db, float *d_dbias, const void *d_dout,
+                                          const void *d_a, const void *d_b, const void *d_preact,
+                                          void *d_dpre, int M, int N, int K, int activation, void *stream) {
+  return backward(d_da, d_db, d_dbias, d_dout, d_a, d_b, d_preact, d_dpre, nullptr, 0, M, N, K, activation,
+                  stream, "linear_backward_bf16");
+}
+
+extern "C" int thork_grouped_gemm_bf16(const void *d_a, const void *d_b, void *d_out, const int *d_offsets,
+                                       void *d_preact, int E, int T, int N, int K, int activation,
+                                       int flags, void *stream) {
+  return grouped<KIND_BF16>(d_a, d_b, d_out, d_offsets, d_preact, E, T, N, K, 1.0f, nullptr, activation,
+                            flags, stream, "grouped_gemm_bf16");
+}
+
+extern "C" int thork_grouped_gemm_e4m3(const void *d_a, const void *d_b, void *d_out, const int *d_offsets,
+                                       void *d_preact, int E, int T, int N, int K, float scale_a,
+                                       const float *d_scale_b, int activation, int flags, void *stream) {
+  return grouped<KIND_E4M3>(d_a, d_b, d_out, d_offsets, d_preact, E, T, N, K, scale_a, d_scale_b,
+                            activation, flags, stream, "grouped_gemm_e4m3");
+}
+
+extern "C" int thork_grouped_gemm_backward_bf16(void *d_da, void *d_db, const void *d_dout, const void *d_a,
+                                                const void *d_b, const int *d_offsets, const void *d_preact,
+                                                void *d_dpre, int E, int T, int N, int K, int activation,
+                                                void *stream) {
+  int rc;
+  if ((rc = check_groups(E, d_offsets, "grouped_gemm_backward_bf16"))) return rc;
+  return backward(d_da, d_db, nullptr, d_dout, d_a, d_b, d_preact, d_dpre, d_offsets, E, T, N, K,
+                  activation, stream, "grouped_gemm_backward_bf16");
+}

@@ -9,6 +9,10 @@ int thork_cuda_error(cudaError_t e, const char *what);
 int thork_encode_tmap_2d(void *out128, int dtype, const void *base, uint64_t rows, uint64_t cols,
                          uint64_t row_stride_bytes, uint32_t box_rows, uint32_t box_cols,
                          int swizzle_bytes);
+// Dense 3-D tensor map (d0 innermost, in elements) with a box0 x box1 x 1 box
+// and 128-byte swizzle; out128 is 64-byte aligned.
+int thork_encode_tmap_3d(void *out128, int dtype, const void *base, uint64_t d0, uint64_t d1, uint64_t d2,
+                         uint32_t box0, uint32_t box1);
 // Per-device status word (4 x u32, cudaMalloc'd and zeroed on first use).
 int thork_status_word(unsigned **d_status);
 // Cached multiprocessor count of the current device.

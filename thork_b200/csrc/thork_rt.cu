@@ -530,6 +530,21 @@ extern "C" int thork_launch(void *function, const unsigned grid[3], const unsign
 // ---------------------------------------------------------------------------
 // TMA descriptors
 // ---------------------------------------------------------------------------
+namespace {
+int tmap_dtype(int dtype, CUtensorMapDataType *t) {
+  switch (dtype) {
+    case THORK_DT_U8:
+    case THORK_DT_E4M3: *t = CU_TENSOR_MAP_DATA_TYPE_UINT8; return THORK_OK;
+    case THORK_DT_U16: *t = CU_TENSOR_MAP_DATA_TYPE_UINT16; return THORK_OK;
+    case THORK_DT_BF16: *t = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16; return THORK_OK;
+    case THORK_DT_F16: *t = CU_TENSOR_MAP_DATA_TYPE_FLOAT16; return THORK_OK;
+    case THORK_DT_U32: *t = CU_TENSOR_MAP_DATA_TYPE_UINT32; return THORK_OK;
+    case THORK_DT_F32: *t = CU_TENSOR_MAP_DATA_TYPE_FLOAT32; return THORK_OK;
+    default: return thork_set_error(THORK_ERR_INVALID, "tensor map: unknown dtype %d", dtype);
+  }
+}
+}  // namespace
+
 int thork_encode_tmap_2d(void *out128, int dtype, const void *base, uint64_t rows, uint64_t cols,
                          uint64_t row_stride_bytes, uint32_t box_rows, uint32_t box_cols,
                          int swizzle_bytes) {
@@ -539,16 +554,7 @@ int thork_encode_tmap_2d(void *out128, int dtype, const void *base, uint64_t row
   int rc = driver_api(&d);
   if (rc) return rc;
   CUtensorMapDataType t;
-  switch (dtype) {
-    case THORK_DT_U8:
-    case THORK_DT_E4M3: t = CU_TENSOR_MAP_DATA_TYPE_UINT8; break;
-    case THORK_DT_U16: t = CU_TENSOR_MAP_DATA_TYPE_UINT16; break;
-    case THORK_DT_BF16: t = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16; break;
-    case THORK_DT_F16: t = CU_TENSOR_MAP_DATA_TYPE_FLOAT16; break;
-    case THORK_DT_U32: t = CU_TENSOR_MAP_DATA_TYPE_UINT32; break;
-    case THORK_DT_F32: t = CU_TENSOR_MAP_DATA_TYPE_FLOAT32; break;
-    default: return thork_set_error(THORK_ERR_INVALID, "tensor map: unknown dtype %d", dtype);
-  }
+  if ((rc = tmap_dtype(dtype, &t))) return rc;
   CUtensorMapSwizzle sw;
   switch (swizzle_bytes) {
     case 0: sw = CU_TENSOR_MAP_SWIZZLE_NONE; break;
@@ -564,6 +570,27 @@ int thork_encode_tmap_2d(void *out128, int dtype, const void *base, uint64_t row
   CUresult r = d->cuTensorMapEncodeTiled(
       reinterpret_cast<CUtensorMap *>(out128), t, 2, const_cast<void *>(base), dims, strides, box,
       estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return drv_error(r, "cuTensorMapEncodeTiled");
+  return THORK_OK;
+}
+
+int thork_encode_tmap_3d(void *out128, int dtype, const void *base, uint64_t d0, uint64_t d1, uint64_t d2,
+                         uint32_t box0, uint32_t box1) {
+  DriverApi *d;
+  int rc = driver_api(&d);
+  if (rc) return rc;
+  CUtensorMapDataType t;
+  if ((rc = tmap_dtype(dtype, &t))) return rc;
+  const uint64_t elem = dtype == THORK_DT_E4M3 || dtype == THORK_DT_U8 ? 1
+                        : dtype == THORK_DT_U32 || dtype == THORK_DT_F32 ? 4 : 2;
+  cuuint64_t dims[3] = {d0, d1, d2};
+  cuuint64_t strides[2] = {d0 * elem, d0 * d1 * elem};
+  cuuint32_t box[3] = {box0, box1, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = d->cuTensorMapEncodeTiled(
+      reinterpret_cast<CUtensorMap *>(out128), t, 3, const_cast<void *>(base), dims, strides, box, estr,
+      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return drv_error(r, "cuTensorMapEncodeTiled");
   return THORK_OK;

@@ -3,6 +3,7 @@ argument binding with the reference's copy-in / launch / synchronise /
 copy-back-written semantics (``src/thork/runtime.py:625-700``), around a
 C-ABI entry point of libthork_rt.so instead of a traced kernel."""
 
+import math
 from typing import Callable, List, Optional, Sequence, Tuple
 
 import numpy as np
@@ -81,6 +82,75 @@ def run(specs: Sequence[ArgSpec], args: Sequence, launch: Callable[[List[int], O
         for a, ptr in back:
             rt.copy_dtoh(a, ptr, s, sync=False)
         if sync or back:
+            s.synchronize()
+    finally:
+        for b in owned:
+            b.free()
+
+
+class Operand:
+    """One array argument of an operator that may be left out: its name,
+    element type, shape and whether the call writes it (``partly``: not all of
+    it, so that a host array's contents go in as well)."""
+
+    __slots__ = ("name", "dtype", "shape", "count", "written", "partly", "_ok")
+
+    def __init__(self, name: str, dtype: dt.Dtype, shape: Tuple[int, ...], written: bool = False,
+                 partly: bool = False):
+        self.name, self.dtype, self.shape = name, dtype, tuple(shape)
+        self.count = math.prod(shape)
+        self.written, self.partly = written, partly
+        self._ok = set()  # storage dtypes that have been accepted before
+
+    def check(self, a, dev: int) -> None:
+        host = isinstance(a, np.ndarray)
+        if not host and not isinstance(a, rt.DeviceArray):
+            raise TypeError(f"Argument for '{self.name}' must be a numpy array or a DeviceArray, got "
+                            f"{type(a).__name__}")
+        if a.dtype not in self._ok:
+            if not dt.storage_compatible(a.dtype, self.dtype):
+                raise TypeError(f"Argument for '{self.name}' has dtype {a.dtype}, expected "
+                                f"{self.dtype.name}")
+            self._ok.add(a.dtype)
+        if math.prod(a.shape) != self.count:
+            raise ValueError(f"Argument for '{self.name}' has shape {tuple(a.shape)}, expected "
+                             f"{self.shape}")
+        if host:
+            if not a.flags["C_CONTIGUOUS"]:
+                raise ValueError(f"Argument for '{self.name}' must be C-contiguous")
+        elif a.buffer._dev != dev:
+            raise ValueError(f"Argument for '{self.name}' is on device {a.buffer._dev}; the call runs on "
+                             f"device {dev}")
+
+
+def run_operands(operands: Sequence[Operand], args: Sequence, launch: Callable, what: str,
+                 stream: Optional["rt.Stream"] = None, sync: bool = True) -> None:
+    """Like ``run`` for operands that may be ``None``: checks ``args``, calls
+    ``launch(pointers, stream_handle)`` with ``None`` for those left out, and
+    copies host arrays in and written ones back."""
+    dev = rt.get_device()
+    s = stream if stream is not None else rt._dispatch_stream()
+    ptrs, owned, back = [], [], []
+    try:
+        for o, a in zip(operands, args):
+            if a is None:
+                ptrs.append(None)
+                continue
+            o.check(a, dev)
+            if isinstance(a, rt.DeviceArray):
+                ptrs.append(a.buffer.ptr)
+                continue
+            buf = rt.DeviceBuffer(a.nbytes)
+            owned.append(buf)
+            ptrs.append(buf.ptr)
+            if not o.written or o.partly:
+                rt.copy_htod(buf.ptr, a, s, sync=False)
+            if o.written:
+                back.append((a, buf.ptr))
+        rt.check(launch(ptrs, s.handle), what)
+        for a, ptr in back:
+            rt.copy_dtoh(a, ptr, s, sync=False)
+        if sync or owned:
             s.synchronize()
     finally:
         for b in owned:

@@ -105,6 +105,12 @@ _SIGNATURES = {
     "thork_gemm_bf16_allgather_mc": [_vp, _vp, _vp, _i, _i, _i, _i, _vp],
     "thork_gemm_e4m3_allgather_mc": [_vp, _vp, _vp, _i, _i, _i, _i, ctypes.c_float,
                                      ctypes.c_float, _vp],
+    "thork_linear_bf16": [_vp] * 6 + [_i] * 5 + [_vp],
+    "thork_linear_e4m3": [_vp] * 6 + [_i] * 3 + [ctypes.c_float] * 2 + [_i] * 2 + [_vp],
+    "thork_linear_backward_bf16": [_vp] * 8 + [_i] * 4 + [_vp],
+    "thork_grouped_gemm_bf16": [_vp] * 5 + [_i] * 6 + [_vp],
+    "thork_grouped_gemm_e4m3": [_vp] * 5 + [_i] * 4 + [ctypes.c_float, _vp] + [_i] * 2 + [_vp],
+    "thork_grouped_gemm_backward_bf16": [_vp] * 8 + [_i] * 5 + [_vp],
     "thork_mc_supported": [ctypes.POINTER(_i)],
     "thork_mc_create": [_sz, _i, _pvp, ctypes.POINTER(_i), ctypes.POINTER(_sz)],
     "thork_mc_import": [_i, _sz, _pvp],
@@ -246,6 +252,17 @@ class Stream:
         h = ctypes.c_void_p()
         check(lib().thork_stream_create(ctypes.byref(h)), "stream create")
         self.handle = h.value
+        self._owned = True
+
+    @classmethod
+    def from_handle(cls, handle: int) -> "Stream":
+        """The stream of another library, by its ``cudaStream_t`` (0 is the
+        legacy default stream).  It stays that library's: ``close`` leaves it
+        alone."""
+        s = cls.__new__(cls)
+        s.handle = int(handle) or None
+        s._owned = False
+        return s
 
     def synchronize(self) -> None:
         check(lib().thork_stream_synchronize(self.handle), "stream synchronize")
@@ -256,7 +273,8 @@ class Stream:
 
     def close(self) -> None:
         if self.handle:
-            lib().thork_stream_destroy(self.handle)
+            if self._owned:
+                lib().thork_stream_destroy(self.handle)
             self.handle = None
 
 
@@ -415,6 +433,26 @@ def to_device(arr: np.ndarray) -> DeviceArray:
 def empty(shape, dtype) -> DeviceArray:
     get_device()
     return DeviceArray(shape, dtype)
+
+
+class _Borrowed:
+    """Device memory that another library owns (kept alive through ``owner``)."""
+
+    __slots__ = ("ptr", "nbytes", "_owner", "_dev")
+
+    def __init__(self, ptr: int, nbytes: int, owner):
+        self.ptr, self.nbytes, self._owner, self._dev = int(ptr), int(nbytes), owner, get_device()
+
+    def free(self) -> None:
+        self.ptr, self._owner = 0, None
+
+
+def wrap_pointer(ptr: int, shape, dtype, owner=None) -> DeviceArray:
+    """A DeviceArray over C-contiguous device memory of another library, on
+    the current device (for example a torch tensor's ``data_ptr()``, with the
+    tensor as ``owner`` so that it outlives the array)."""
+    n = int(np.prod(shape, dtype=np.int64)) * np.dtype(dtype).itemsize
+    return DeviceArray(shape, dtype, buffer=_Borrowed(ptr, n, owner))
 
 
 def copy_htod(d_ptr: int, arr: np.ndarray, stream: Optional[Stream] = None, sync: bool = True) -> None:
