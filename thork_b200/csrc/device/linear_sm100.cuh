@@ -2,8 +2,9 @@
 // with bias, activation and residual in the epilogue, and the same products
 // grouped by expert with ragged sizes, forward and backward.
 //
-//   pair_kernel   persistent CTA pairs (tcgen05 cta_group::2), 256 x BN tiles:
-//                 the tensor-bound products (many rows; both gradients)
+//   rows_kernel   persistent CTA pairs (tcgen05 cta_group::2), tiles of 256
+//                 columns by up to 256 rows: products of many rows
+//   outer_kernel  the same for a product over rows: the weights' gradient
 //   swap_kernel   one 128 x BN tile per cluster with the weights as the MMA's
 //                 128 rows, the contraction split over the cluster and summed
 //                 through distributed shared memory: few rows, bound by the
@@ -26,8 +27,6 @@ using namespace thork::dev;
 
 enum : int { KIND_BF16 = 0, KIND_E4M3 = 1 };
 enum : int { ACT_NONE = 0, ACT_RELU = 1, ACT_GELU = 2, ACT_GELU_TANH = 3, ACT_SILU = 4 };
-// what the product's groups divide: nothing, the output's rows, or the contraction
-enum : int { DENSE = 0, GROUP_ROWS = 1, GROUP_K = 2 };
 
 constexpr int kMaxGroups = 1024;
 
@@ -49,7 +48,7 @@ struct Epilogue {
 
 struct GemmArgs {
   Epilogue epi;
-  int GM, GN, GK;      // extents of the (per-group) product; GROUP_ROWS: GM = buffer rows
+  int GM, GN, GK;      // extents of the (per-group) product; grouped rows: GM = buffer rows
   const int *offsets;  // [groups + 1] row offsets, or null
   int groups, rows;    // groups, rows of the buffer that the offsets divide
   int w_static;        // swap_kernel: no earlier launch writes the weights
@@ -99,11 +98,36 @@ __device__ __forceinline__ float bf16_lo(u32 w) { return __uint_as_float(w << 16
 __device__ __forceinline__ float bf16_hi(u32 w) { return __uint_as_float(w & 0xFFFF0000u); }
 
 // ---------------------------------------------------------------- activations
-// gelu_tanh is written z * sigmoid(2u), silu z * sigmoid(z): one exponential
-// and one division each, with a relative error of a few 2^-22, far below the
-// bf16 rounding of the output.  A NaN stays a NaN (relu included).
+// silu is z * sigmoid(z) and gelu_tanh z * sigmoid(2u): one exponential and one
+// division each, off by a few 2^-22 of the value.  The normal distribution
+// function of gelu takes Abramowitz and Stegun's rational approximation
+// 7.1.26 of erf (absolute error 1.5e-7), because its exponential is the
+// density's, which the slope needs as well: with erff and expf the slope
+// kernel was bound by its instructions (126 us for 4096 x 14336 against 54 us
+// of traffic).  All of it is far below the bf16 rounding of what is stored.
+// A NaN stays a NaN (relu included).
 __device__ __forceinline__ float gelu_tanh_2u(float z) {
   return 1.5957691216057308f * z * (1.0f + 0.044715f * z * z);
+}
+
+// 1 / x to within 2^-23 or so; 0 for infinity.
+__device__ __forceinline__ float reciprocal(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float sigmoid(float z) { return reciprocal(1.0f + __expf(-z)); }
+
+// Phi(z), and bell = exp(-z^2 / 2).
+__device__ __forceinline__ float normal_cdf(float z, float &bell) {
+  bell = __expf(-0.5f * z * z);
+  const float t = reciprocal(fmaf(0.3275911f * 0.7071067811865476f, fabsf(z), 1.0f));
+  // half of the approximation's polynomial
+  const float poly =
+      t * (0.127414796f + t * (-0.142248368f + t * (0.7107068705f + t * (-0.7265760135f + t * 0.5307027145f))));
+  const float tail = poly * bell;  // Phi(-|z|)
+  return z < 0.0f ? tail : 1.0f - tail;
 }
 
 template <int N>
@@ -113,33 +137,46 @@ __device__ __forceinline__ void act_forward(float (&v)[N], int act) {
     for (int i = 0; i < N; ++i) v[i] = v[i] <= 0.0f ? 0.0f : v[i];
   } else if (act == ACT_GELU) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = 0.5f * v[i] * (1.0f + erff(v[i] * 0.7071067811865476f));
+    for (int i = 0; i < N; ++i) {
+      float bell;
+      v[i] *= normal_cdf(v[i], bell);
+    }
   } else if (act == ACT_GELU_TANH) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = __fdividef(v[i], 1.0f + __expf(-gelu_tanh_2u(v[i])));
+    for (int i = 0; i < N; ++i) v[i] *= sigmoid(gelu_tanh_2u(v[i]));
   } else if (act == ACT_SILU) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = __fdividef(v[i], 1.0f + __expf(-v[i]));
+    for (int i = 0; i < N; ++i) v[i] *= sigmoid(v[i]);
   }
 }
 
-// Derivative of the activation at z.
-__device__ __forceinline__ float act_slope(float z, int act) {
-  if (act == ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
-  if (act == ACT_GELU) {
-    const float cdf = 0.5f * (1.0f + erff(z * 0.7071067811865476f));
-    return cdf + z * 0.3989422804014327f * expf(-0.5f * z * z);
+// v[i] *= derivative of the activation at z[i].
+template <int N>
+__device__ __forceinline__ void act_backward(float (&v)[N], const float (&z)[N], int act) {
+  if (act == ACT_RELU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] *= z[i] > 0.0f ? 1.0f : 0.0f;
+  } else if (act == ACT_GELU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float bell;
+      const float cdf = normal_cdf(z[i], bell);
+      v[i] *= cdf + z[i] * 0.3989422804014327f * bell;
+    }
+  } else if (act == ACT_GELU_TANH) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      // d(2u)/dz = 2 sqrt(2/pi) (1 + 3 * 0.044715 z^2)
+      const float p = sigmoid(gelu_tanh_2u(z[i]));
+      v[i] *= p + z[i] * p * (1.0f - p) * 1.5957691216057308f * (1.0f + 0.134145f * z[i] * z[i]);
+    }
+  } else if (act == ACT_SILU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float p = sigmoid(z[i]);
+      v[i] *= p * (1.0f + z[i] * (1.0f - p));
+    }
   }
-  if (act == ACT_GELU_TANH) {
-    const float p = 1.0f / (1.0f + expf(-gelu_tanh_2u(z)));
-    // d(2u)/dz = 2 sqrt(2/pi) (1 + 3 * 0.044715 z^2)
-    return p + z * p * (1.0f - p) * 1.5957691216057308f * (1.0f + 0.134145f * z * z);
-  }
-  if (act == ACT_SILU) {
-    const float p = 1.0f / (1.0f + expf(-z));
-    return p * (1.0f + z * (1.0f - p));
-  }
-  return 1.0f;
 }
 
 // ---------------------------------------------------------------- groups
@@ -183,226 +220,574 @@ __device__ __forceinline__ void scan_groups(const int *offsets, int groups, int 
 }
 
 // ===========================================================================
-// pair_kernel
+// rows_kernel
 // ===========================================================================
-// A cluster of two CTAs computes 256 x BN tiles; CTA r holds rows
-// [128 r, 128 r + 128) of the A tile and columns [BN/2 r, BN/2 (r + 1)) of the
-// B tile, and owns the tile's accumulator rows of its half.  Warps: 0 TMA
-// producer, 1 MMA issuer (leader only), 2..9 epilogue (two warps per TMEM
-// lane quadrant, each half of the tile's 64-column slices), 10 (GROUP_K
-// only) zeroes the rows behind a group's end in its last k-block.
+// out[m, n] = act(sum_k X[m, k] W[k, n] ...) for many rows.  A cluster of two
+// CTAs computes tiles of 256 columns n by up to 256 rows m, as the transpose:
+// the weights are the MMA's M dimension (CTA r holds columns
+// [128 r, 128 r + 128)), the rows its N dimension (CTA r holds one half of the
+// tile's rows).  The N dimension of an instruction may be any multiple of 32,
+// so a tile has as many rows as there are, in units of 64: a group's rows, or
+// a product's, are dealt out in even tiles of at most four units, and no
+// multiplication is spent on rows of another group.  With rows as the M
+// dimension every group would round up to 256 rows.
 //
-// GROUP_K needs that because the contraction runs over a group's rows, whose
-// count is any number: the last k-block also loads rows of the next group, or
-// rows behind the last one, whose values (NaN among them) must not count.
-// Those rows are whole 128-byte lines of both MN-major operands.  Such a
-// block's loads complete on a barrier of the CTA's own; warp 10 zeroes the
-// lines and, once both CTAs have, releases the block to the MMA thread.
-template <int KIND_, int BN_, int STAGES_, bool A_MN_, bool B_MN_, int MODE_>
-struct PairCfg {
-  static constexpr int KIND = KIND_, BN = BN_, STAGES = STAGES_, MODE = MODE_;
-  static constexpr bool A_MN = A_MN_, B_MN = B_MN_;
+// Persistent: pair i takes tiles i, i + pairs, ...; the tiles of the last,
+// partial wave are split by rows into as many pieces as there are pairs for
+// (4096^3: 256 tiles are 3.46 waves; the last 34 become 68 halves).
+//
+// Warps: 0 TMA producer, 1 MMA issuer (leader only), 2..9 epilogue: two warps
+// per TMEM lane quadrant, taking the tile's 32-row slices in turn.
+template <int KIND_, bool W_MN_, bool GROUPED_>
+struct RowsCfg {
+  static constexpr int KIND = KIND_, STAGES = 6;
+  static constexpr bool W_MN = W_MN_, GROUPED = GROUPED_;
   static constexpr int ELEM = KIND == KIND_BF16 ? 2 : 1;
-  static constexpr int BM = 128;  // rows per CTA
-  static constexpr int BNH = BN / 2;
+  static constexpr int BNC = 128;  // columns per CTA
+  static constexpr int UNIT = 64, MAX_UNITS = 4;
+  static constexpr int BOX_ROWS = UNIT / 2;  // a CTA's half of a unit, one TMA box
   static constexpr int BK = 128 / ELEM;
-  static constexpr int CHUNK = 128 / ELEM;  // MN elements per 128-byte line
+  static constexpr int CHUNK = 128 / ELEM;
   static constexpr int UMMA_K = 32 / ELEM;
-  static constexpr int A_BYTES = BM * 128, B_BYTES = BNH * 128;
-  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int TMEM_COLS = 2 * BN;
+  static constexpr int W_BYTES = BNC * 128, BOX_BYTES = BOX_ROWS * 128;
+  static constexpr int STAGE_BYTES = W_BYTES + MAX_UNITS * BOX_BYTES;
+  static constexpr int TMEM_COLS = 2 * UNIT * MAX_UNITS;
   static constexpr int EPI_WARPS = 8;
-  static constexpr int THREADS = 32 * (2 + EPI_WARPS + (MODE == GROUP_K ? 1 : 0));
-  static constexpr int GROUP_M = 8;  // pair-tile rows per raster group
-  // shared memory: stages | staging (4 KiB per epilogue warp) | barriers | group table
+  static constexpr int THREADS = 32 * (2 + EPI_WARPS);
+  static constexpr int RASTER = 8;  // row tiles walked column by column
   static constexpr int STG_OFF = STAGES * STAGE_BYTES;
-  static constexpr int BAR_OFF = STG_OFF + EPI_WARPS * 4096;
-  static constexpr int NBARS = 2 * STAGES + 5 + (MODE == GROUP_K ? 2 * STAGES : 0);
+  static constexpr int BAR_OFF = STG_OFF + EPI_WARPS * 2048;
+  static constexpr int NBARS = 2 * STAGES + 5;
   static constexpr int TAB_OFF = BAR_OFF + NBARS * 8 + 16;
-  static constexpr int TAB_BYTES =
-      MODE == DENSE ? 0 : (kMaxGroups + 1) * 4 * (MODE == GROUP_ROWS ? 2 : 1);
+  static constexpr int TAB_BYTES = GROUPED ? (kMaxGroups + 1) * 8 : 0;
   static constexpr int SMEM_BYTES = 1024 + TAB_OFF + TAB_BYTES;
+  // without the N field, which is the tile's
   static constexpr u32 IDESC =
-      make_idesc(KIND == KIND_BF16 ? 1u : 0u, KIND == KIND_BF16 ? 1u : 0u, A_MN, B_MN, 256, BN);
-  static_assert(BN == 256 || BN == 128, "whole 64-column slices for both epilogue halves");
-  static_assert(!B_MN || BNH % CHUNK == 0, "per-CTA B columns are whole 128-byte lines");
+      make_idesc(KIND == KIND_BF16 ? 1u : 0u, KIND == KIND_BF16 ? 1u : 0u, W_MN, false, 256, 0);
   static_assert(SMEM_BYTES <= 232448, "shared memory budget exceeded");
 };
 
-struct Tile {
-  int m0, n0;     // first output row (of the pair) and column
-  int row_end;    // rows from here on belong to another group
-  int grp;        // group, 0 when dense
-  int k0;         // GROUP_K: first row of the contraction
-  int nkb, tail;  // k-blocks; GROUP_K: valid rows of the last one, 0 when whole
+template <int N>
+struct Const {
+  static constexpr int value = N;
+};
+
+struct RowTile {
+  int m0, row_end;  // first row; rows from here on belong to another tile or group
+  int n0;           // first column (of the pair)
+  int units;        // 64-row units
+  int grp;
 };
 
 // The pair's tiles in order; every role walks the same sequence.
 template <class C>
-struct Walk {
+struct RowWalk {
   const GemmArgs &g;
   const int *tab_off, *tab_tile;
-  int t, step, total, grp, ntn;
+  int i, step, whole, pieces, items, grp, ntn;
 
-  __device__ __forceinline__ Walk(const GemmArgs &g_, const int *o, const int *tl)
-      : g(g_), tab_off(o), tab_tile(tl), t(blockIdx.x / 2), step(gridDim.x / 2), grp(0) {
-    ntn = (g.GN + C::BN - 1) / C::BN;
-    const int ntm = (g.GM + 255) / 256;
-    total = C::MODE == GROUP_ROWS ? tab_tile[g.groups] * ntn
-                                  : ntm * ntn * (C::MODE == GROUP_K ? g.groups : 1);
+  __device__ __forceinline__ RowWalk(const GemmArgs &g_, const int *o, const int *tl)
+      : g(g_), tab_off(o), tab_tile(tl), i(blockIdx.x / 2), step(gridDim.x / 2), grp(0) {
+    ntn = (g.GN + 2 * C::BNC - 1) / (2 * C::BNC);
+    const int total = (C::GROUPED ? tab_tile[g.groups] : row_tiles(g.GM)) * ntn;
+    const int rest = total % step;
+    whole = total - rest;
+    pieces = rest ? min(C::MAX_UNITS, step / rest) : 1;
+    items = whole + rest * pieces;
+  }
+  static __device__ __forceinline__ int row_tiles(int rows) {
+    return (rows + C::UNIT * C::MAX_UNITS - 1) / (C::UNIT * C::MAX_UNITS);
   }
 
-  // raster: groups of GROUP_M tile rows walked column by column, so that the
-  // tiles in flight share operand panels in L2
-  __device__ __forceinline__ void raster(int local, int ntm, Tile &x) const {
-    const int per = C::GROUP_M * ntn;
-    const int q = local / per, first = q * C::GROUP_M, r = local - q * per;
-    const int rows = min(ntm - first, C::GROUP_M);
-    x.m0 = (first + r % rows) * 256;
-    x.n0 = r / rows * C::BN;
-  }
-
-  __device__ __forceinline__ bool next(Tile &x) {
-    if (t >= total) return false;
-    if (C::MODE == GROUP_ROWS) {
-      while (t >= tab_tile[grp + 1] * ntn) ++grp;
-      const int first = tab_tile[grp];
-      raster(t - first * ntn, tab_tile[grp + 1] - first, x);
-      x.m0 += tab_off[grp];
-      x.row_end = tab_off[grp + 1];
-      x.grp = grp;
-    } else {
-      const int ntm = (g.GM + 255) / 256;
-      x.grp = C::MODE == GROUP_K ? t / (ntm * ntn) : 0;
-      raster(t - x.grp * ntm * ntn, ntm, x);
-      x.row_end = g.GM;
+  __device__ __forceinline__ bool next(RowTile &x) {
+    for (; i < items; i += step) {
+      int t = i, piece = 0, parts = 1;
+      if (i >= whole && pieces > 1) {
+        const int r = i - whole;
+        t = whole + r / pieces;
+        piece = r - r / pieces * pieces;
+        parts = pieces;
+      }
+      int first = 0, base = 0, rows = g.GM, ntm;
+      if (C::GROUPED) {
+        while (t >= tab_tile[grp + 1] * ntn) ++grp;
+        first = tab_tile[grp];
+        ntm = tab_tile[grp + 1] - first;
+        base = tab_off[grp];
+        rows = tab_off[grp + 1] - base;
+      } else {
+        ntm = row_tiles(rows);
+      }
+      const int local = t - first * ntn, per = C::RASTER * ntn;
+      const int q = local / per, r = local - q * per;
+      const int band = min(ntm - q * C::RASTER, C::RASTER);
+      const int tn = r / band, tm = q * C::RASTER + r - tn * band;
+      // the row tile's units, and of those the piece's
+      const int units = min((rows - tm * (C::UNIT * C::MAX_UNITS) + C::UNIT - 1) / C::UNIT, C::MAX_UNITS);
+      const int p0 = units * piece / parts, p1 = units * (piece + 1) / parts;
+      if (p1 == p0) continue;
+      const int row = tm * (C::UNIT * C::MAX_UNITS);
+      x.m0 = base + row + p0 * C::UNIT;
+      x.row_end = base + min(rows, row + p1 * C::UNIT);
+      x.n0 = tn * 2 * C::BNC;
+      x.units = p1 - p0;
+      x.grp = C::GROUPED ? grp : 0;
+      i += step;
+      return true;
     }
-    if (C::MODE == GROUP_K) {
-      x.k0 = tab_off[x.grp];
-      const int len = tab_off[x.grp + 1] - x.k0;
-      x.nkb = (len + C::BK - 1) / C::BK;
-      x.tail = len % C::BK;
-    } else {
-      x.k0 = 0;
-      x.nkb = (g.GK + C::BK - 1) / C::BK;
-      x.tail = 0;
-    }
-    t += step;
-    return true;
+    return false;
   }
 };
 
-// One warp's 32 accumulator rows x 64 columns of residual, 16 bytes per lane
-// and step: lane covers chunk lane % 8 of row 4 it + lane / 8.
-__device__ __forceinline__ void load_residual(uint4 (&res)[8], const Epilogue &p, int row0, int row_end,
-                                              int col0, int lane) {
-  const int col = col0 + (lane & 7) * 8;
+// A warp's block of the output: 32 columns n (TMEM lanes) by 32 rows m (TMEM
+// columns).  tcgen05.ld.16x256b delivers it as 8 x 8 fragments of (n, m), and
+// stmatrix.trans writes such fragments as (m, n): one instruction per four
+// fragments turns the accumulator's columns into the output's rows.
+//
+// Fragment values: f[h][4 j + 2 e + i] is column n = 16 h + 8 e + lane / 4,
+// row m = 8 j + 2 (lane % 4) + i.  The staging block is 32 rows of 64 bytes;
+// 16-byte chunk c of row r lies at chunk c ^ (r / 2 % 4), which spreads the
+// eight rows of a fragment over all banks.
+__device__ __forceinline__ void tmem_ld_16x256b_x4(u32 taddr, u32 (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+
+// Address that this lane gives a matrix instruction over the four column
+// blocks (chunks) of rows [8 j, 8 j + 8): row 8 j + lane % 8, chunk lane / 8.
+__device__ __forceinline__ u32 block_addr(u32 stg, int j, int lane) {
+  const int r = 8 * j + (lane & 7);
+  return stg + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) * 16);
+}
+
+__device__ __forceinline__ void put_block(const float (&f)[2][16], u32 stg, int lane) {
 #pragma unroll
-  for (int it = 0; it < 8; ++it) {
-    const int row = row0 + 4 * it + (lane >> 3);
-    res[it] = make_uint4(0, 0, 0, 0);
-    if (row < row_end && col < p.cols)
-      // an ordinary load: out may be the residual itself
-      res[it] = *reinterpret_cast<const uint4 *>(p.residual + static_cast<long long>(row) * p.cols + col);
+  for (int j = 0; j < 4; ++j)
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(
+                     block_addr(stg, j, lane)),
+                 "r"(pack_bf16x2(f[0][4 * j], f[0][4 * j + 1])), "r"(pack_bf16x2(f[0][4 * j + 2], f[0][4 * j + 3])),
+                 "r"(pack_bf16x2(f[1][4 * j], f[1][4 * j + 1])), "r"(pack_bf16x2(f[1][4 * j + 2], f[1][4 * j + 3]))
+                 : "memory");
+}
+
+__device__ __forceinline__ void add_block(float (&f)[2][16], u32 stg, int lane) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    u32 w[4];
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                 : "r"(block_addr(stg, j, lane))
+                 : "memory");
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        f[h][4 * j + 2 * e] += bf16_lo(w[2 * h + e]);
+        f[h][4 * j + 2 * e + 1] += bf16_hi(w[2 * h + e]);
+      }
   }
 }
 
-__device__ __forceinline__ void store_slice(const unsigned char *stg, unsigned short *out, int cols,
-                                            int row0, int row_end, int col0, int lane) {
-  const int chunk = lane & 7, col = col0 + chunk * 8;
+// The block's rows in global memory, 16 bytes per lane and step: lane covers
+// chunk lane % 4 of row 8 it + lane / 4.
+__device__ __forceinline__ void load_block(uint4 (&v)[4], const unsigned short *src, int cols, int row0,
+                                           int row_end, int col0, int lane) {
+  const int col = col0 + (lane & 3) * 8;
 #pragma unroll
-  for (int it = 0; it < 8; ++it) {
-    const int r = 4 * it + (lane >> 3), row = row0 + r;
-    const uint4 v = *reinterpret_cast<const uint4 *>(stg + r * 128 + ((chunk ^ (r & 7)) * 16));
+  for (int it = 0; it < 4; ++it) {
+    const int row = row0 + 8 * it + (lane >> 2);
+    v[it] = make_uint4(0, 0, 0, 0);
+    // an ordinary load: out may be the residual itself
     if (row < row_end && col < cols)
-      st_global_v4(out + static_cast<long long>(row) * cols + col, v.x, v.y, v.z, v.w);
+      v[it] = *reinterpret_cast<const uint4 *>(src + static_cast<long long>(row) * cols + col);
   }
 }
 
-// Epilogue of 32 rows x 64 columns (TMEM lanes of t_row, or zeros).  Thread =
-// row: the accumulator arrives with a row's columns in one thread, and leaves
-// through this warp's 4 KiB staging slice (row = lane, 16-byte chunks XOR the
-// row, so both directions are free of bank conflicts) as whole 128-byte
-// lines.  The residual takes the same way in: loaded in whole lines, laid
-// into the slice, picked up by the row's thread and added in fp32.
-__device__ __forceinline__ void epilogue_slice(const Epilogue &p, u32 t_row, bool zero, float alpha,
-                                               int row0, int row_end, int col0,
-                                               const uint4 (&res)[8], unsigned char *stg, int lane) {
-  float v[64];
-  if (zero) {
+__device__ __forceinline__ uint4 *staged(unsigned char *stg, int it, int lane) {
+  const int r = 8 * it + (lane >> 2);
+  return reinterpret_cast<uint4 *>(stg + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) * 16));
+}
+
+__device__ __forceinline__ void store_block(unsigned char *stg, unsigned short *dst, int cols, int row0,
+                                            int row_end, int col0, int lane) {
+  const int col = col0 + (lane & 3) * 8;
 #pragma unroll
-    for (int i = 0; i < 64; ++i) v[i] = 0.0f;
-  } else {
-    u32 a[32], b[32];
-    tmem_ld_32x32b_x32(t_row, a);
-    tmem_ld_32x32b_x32(t_row + 32, b);
-    tmem_wait_ld();
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      v[i] = __uint_as_float(a[i]) * alpha;
-      v[32 + i] = __uint_as_float(b[i]) * alpha;
-    }
+  for (int it = 0; it < 4; ++it) {
+    const int row = row0 + 8 * it + (lane >> 2);
+    const uint4 v = *staged(stg, it, lane);
+    // cols is a multiple of 8, so a 16-byte chunk is wholly in or out
+    if (row < row_end && col < cols)
+      st_global_v4(dst + static_cast<long long>(row) * cols + col, v.x, v.y, v.z, v.w);
   }
-  if (p.bias) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      // cols is a multiple of 8, so an 8-column piece is wholly in or out
-      const int col = col0 + 8 * j;
-      if (col < p.cols) {
-        const uint4 w = __ldg(reinterpret_cast<const uint4 *>(p.bias + col));
-        const u32 x[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          v[8 * j + 2 * h] += bf16_lo(x[h]);
-          v[8 * j + 2 * h + 1] += bf16_hi(x[h]);
-        }
-      }
-    }
-  }
-  auto slot = [&](int j) { return reinterpret_cast<uint4 *>(stg + lane * 128 + ((j ^ (lane & 7)) * 16)); };
-  auto put = [&] {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      *slot(j) = make_uint4(pack_bf16x2(v[8 * j], v[8 * j + 1]), pack_bf16x2(v[8 * j + 2], v[8 * j + 3]),
-                            pack_bf16x2(v[8 * j + 4], v[8 * j + 5]), pack_bf16x2(v[8 * j + 6], v[8 * j + 7]));
-  };
-  if (p.preact) {
-    put();
-    __syncwarp();
-    store_slice(stg, p.preact, p.cols, row0, row_end, col0, lane);
-    __syncwarp();
-  }
-  if (p.residual) {
-#pragma unroll
-    for (int it = 0; it < 8; ++it) {
-      const int r = 4 * it + (lane >> 3);
-      *reinterpret_cast<uint4 *>(stg + r * 128 + (((lane & 7) ^ (r & 7)) * 16)) = res[it];
-    }
-  }
-  act_forward(v, p.act);
-  if (p.residual) {
-    __syncwarp();
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint4 w = *slot(j);
-      const u32 x[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        v[8 * j + 2 * h] += bf16_lo(x[h]);
-        v[8 * j + 2 * h + 1] += bf16_hi(x[h]);
-      }
-    }
-  }
-  put();  // a row's chunks are read and written by its own thread alone
-  __syncwarp();
-  store_slice(stg, p.out, p.cols, row0, row_end, col0, lane);
-  __syncwarp();
 }
 
 template <class C>
 __global__ void __launch_bounds__(C::THREADS, 1)
-    pair_kernel(const __grid_constant__ TensorMap tmap_a, const __grid_constant__ TensorMap tmap_b,
-                const GemmArgs g) {
+    rows_kernel(const __grid_constant__ TensorMap tmap_w, const __grid_constant__ TensorMap tmap_x,
+                const __grid_constant__ TensorMap tmap_xu, const GemmArgs g) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  const u32 raw = smem_u32(smem_raw);
+  const u32 base = (raw + 1023u) & ~1023u;
+  unsigned char *smem = smem_raw + (base - raw);
+  const u32 bars = base + C::BAR_OFF;
+  auto full_bar = [&](int s) { return bars + 8u * s; };
+  auto empty_bar = [&](int s) { return bars + 8u * (C::STAGES + s); };
+  auto tfull_bar = [&](int a) { return bars + 8u * (2 * C::STAGES + a); };
+  auto tempty_bar = [&](int a) { return bars + 8u * (2 * C::STAGES + 2 + a); };
+  const u32 drain_bar = bars + 8u * (2 * C::STAGES + 4);
+  u32 *tmem_slot = reinterpret_cast<u32 *>(smem + C::BAR_OFF + C::NBARS * 8);
+  volatile u32 *abort_flag = tmem_slot + 1;
+  int *tab_off = reinterpret_cast<int *>(smem + C::TAB_OFF);
+  int *tab_tile = tab_off + kMaxGroups + 1;
+  u32 *status = g.epi.status;
+
+  const int warp = threadIdx.x / 32;
+  const int lane = threadIdx.x % 32;
+  const u32 rank = cluster_ctarank();
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(tfull_bar(a), 1);
+      mbar_init(tempty_bar(a), 2 * C::EPI_WARPS);  // both CTAs' epilogue warps, on the leader's
+    }
+    mbar_init(drain_bar, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmap_w);
+    tma_prefetch_desc(&tmap_x);
+    tma_prefetch_desc(&tmap_xu);
+  }
+  if (warp == 1) {
+    tmem_alloc<2>(smem_u32(tmem_slot), C::TMEM_COLS);
+    tmem_relinquish<2>();
+  }
+  if (C::GROUPED && warp == 2) {
+    pdl_wait();  // the offsets may come from the previous kernel of the stream
+    scan_groups(g.offsets, g.groups, g.rows, C::UNIT * C::MAX_UNITS, tab_off, tab_tile,
+                blockIdx.x == 0 ? status : nullptr);
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // both CTAs' barriers are initialised before any remote use
+  tc_fence_after();
+  pdl_launch_dependents();
+  const u32 tmem_base = *tmem_slot;
+  const int nkb = (g.GK + C::BK - 1) / C::BK;
+  pdl_wait();  // the previous kernel of the stream is complete from here on
+
+  if (warp == 0) {
+    // ------------------------------------------------ TMA producer (both CTAs)
+    if (lane == 0) {
+      RowWalk<C> walk(g, tab_off, tab_tile);
+      RowTile x;
+      int s = 0;
+      u32 ph = 0;
+      while (!*abort_flag && walk.next(x)) {
+        const int n = x.n0 + rank * C::BNC, m = x.m0 + rank * x.units * C::BOX_ROWS;
+        const u32 bytes = 2 * (C::W_BYTES + x.units * C::BOX_BYTES);
+        for (int kb = 0; kb < nkb; ++kb) {
+          if (!mbar_wait(empty_bar(s), ph ^ 1u, status, 0x61)) {
+            *abort_flag = 1;
+            break;
+          }
+          const u32 sw = base + s * C::STAGE_BYTES, sx = sw + C::W_BYTES;
+          const u32 fb = mapa_cluster(full_bar(s), 0);
+          if (rank == 0) mbar_arrive_expect_tx(full_bar(s), bytes);
+          if (C::W_MN) {
+#pragma unroll
+            for (int c = 0; c < C::BNC / C::CHUNK; ++c)
+              tma_load_3d_pair(sw + c * C::BK * 128, &tmap_w, fb, n + c * C::CHUNK, kb * C::BK, x.grp);
+          } else {
+            tma_load_3d_pair(sw, &tmap_w, fb, kb * C::BK, n, x.grp);
+          }
+          // a whole tile's rows in one box: a box more costs the TMA unit as
+          // much as eight rows (4096 x 14336 x 4096: 411 us with four boxes
+          // of 32 rows, 389 with one of 128)
+          if (x.units == C::MAX_UNITS)
+            tma_load_3d_pair(sx, &tmap_x, fb, kb * C::BK, m, 0);
+          else
+            for (int u = 0; u < x.units; ++u)
+              tma_load_3d_pair(sx + u * C::BOX_BYTES, &tmap_xu, fb, kb * C::BK, m + u * C::BOX_ROWS, 0);
+          if (++s == C::STAGES) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+      }
+      // drain: every issued load has landed and been read before the CTA exits
+      for (int i = 0; i < C::STAGES; ++i) {
+        if (!mbar_wait(empty_bar(s), ph ^ 1u, status, 0x62)) break;
+        if (++s == C::STAGES) {
+          s = 0;
+          ph ^= 1u;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------ MMA issuer (leader CTA)
+    // all of it in lane 0: a warp-wide step per k-block idles the tensor pipe
+    if (rank == 0 && lane == 0) {
+      RowWalk<C> walk(g, tab_off, tab_tile);
+      RowTile x;
+      int s = 0, it = 0;
+      u32 ph = 0;
+      while (!*abort_flag && walk.next(x)) {
+        const int acc = it & 1;
+        const u32 d_tmem = tmem_base + acc * (C::TMEM_COLS / 2);
+        if (!mbar_wait(tempty_bar(acc), ((it >> 1) & 1) ^ 1u, status, 0x63)) {
+          *abort_flag = 1;
+          break;
+        }
+        tc_fence_after();
+        bool ok = true;
+        // the instruction descriptor as a constant: one that varies at run time
+        // is moved to uniform registers for every instruction
+        auto run = [&](auto units) {
+          constexpr u32 idesc = C::IDESC | (decltype(units)::value * C::UNIT >> 3) << 17;
+          for (int kb = 0; kb < nkb; ++kb) {
+            if (!mbar_wait(full_bar(s), ph, status, 0x64)) {
+              *abort_flag = 1;
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const u32 sw = base + s * C::STAGE_BYTES, sx = sw + C::W_BYTES;
+#pragma unroll
+            for (int k = 0; k < C::BK / C::UMMA_K; ++k) {
+              const u64 ad = C::W_MN ? smem_desc_sw128(sw + k * C::UMMA_K * 128, C::BK * 128, 1024)
+                                     : smem_desc_sw128(sw + k * 32, 16, 1024);
+              const u64 bd = smem_desc_sw128(sx + k * 32, 16, 1024);
+              const u32 accum = (kb > 0 || k > 0) ? 1u : 0u;
+              if (C::KIND == KIND_BF16)
+                mma2_f16_ss(d_tmem, ad, bd, idesc, accum);
+              else
+                mma2_f8f6f4_ss(d_tmem, ad, bd, idesc, accum);
+            }
+            tc_commit2(mapa_cluster(empty_bar(s), 0));
+            tc_commit2(mapa_cluster(empty_bar(s), 1));
+            if (++s == C::STAGES) {
+              s = 0;
+              ph ^= 1u;
+            }
+          }
+        };
+        if (x.units == 4)
+          run(Const<4>());
+        else if (x.units == 3)
+          run(Const<3>());
+        else if (x.units == 2)
+          run(Const<2>());
+        else
+          run(Const<1>());
+        if (!ok || *abort_flag) break;
+        tc_commit2(mapa_cluster(tfull_bar(acc), 0));
+        tc_commit2(mapa_cluster(tfull_bar(acc), 1));
+        ++it;
+      }
+      tc_commit2(mapa_cluster(drain_bar, 0));
+      mbar_wait(drain_bar, 0, status, 0x65);
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------ epilogue (both CTAs)
+    const int q = warp & 3;            // TMEM lane quadrant this warp may access
+    const int half = (warp - 2) >> 2;  // takes slices half, half + 2, ...
+    const Epilogue &p = g.epi;
+    unsigned char *stg = smem + C::STG_OFF + (warp - 2) * 2048;
+    const u32 stg_at = base + C::STG_OFF + (warp - 2) * 2048;
+    RowWalk<C> walk(g, tab_off, tab_tile);
+    RowTile x;
+    int it = 0;
+    while (!*abort_flag && walk.next(x)) {
+      const float alpha = p.group_scale ? p.alpha * __ldg(p.group_scale + x.grp) : p.alpha;
+      const int col0 = x.n0 + rank * C::BNC + q * 32;  // the warp's columns, one per lane
+      const bool live = col0 < p.cols;
+      float bias[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // of columns lane / 4 + 8 i
+      if (p.bias) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int col = col0 + 8 * i + (lane >> 2);
+          if (col < p.cols) bias[i] = __uint_as_float(static_cast<u32>(p.bias[col]) << 16);
+        }
+      }
+      uint4 res[4];
+      if (p.residual && live) load_block(res, p.residual, p.cols, x.m0 + half * 32, x.row_end, col0, lane);
+      const int acc = it & 1;
+      bool ok = true;
+      if (lane == 0) ok = mbar_wait(tfull_bar(acc), (it >> 1) & 1, status, 0x66);
+      if (!__shfl_sync(0xffffffffu, ok ? 1 : 0, 0)) {
+        *abort_flag = 1;
+        break;
+      }
+      tc_fence_after();
+      const u32 t_lane = tmem_base + (static_cast<u32>(q * 32) << 16) + acc * (C::TMEM_COLS / 2);
+      const int slices = live ? x.units * 2 : 0;
+#pragma unroll 1
+      for (int i = half; i < slices; i += 2) {
+        const int row0 = x.m0 + i * 32;
+        if (row0 >= x.row_end) break;
+        u32 lo[16], hi[16];
+        tmem_ld_16x256b_x4(t_lane + i * 32, lo);
+        tmem_ld_16x256b_x4(t_lane + (16u << 16) + i * 32, hi);
+        tmem_wait_ld();
+        float v[2][16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          v[0][j] = fmaf(__uint_as_float(lo[j]), alpha, bias[j >> 1 & 1]);
+          v[1][j] = fmaf(__uint_as_float(hi[j]), alpha, bias[2 + (j >> 1 & 1)]);
+        }
+        if (p.preact) {
+          put_block(v, stg_at, lane);
+          __syncwarp();
+          store_block(stg, p.preact, p.cols, row0, x.row_end, col0, lane);
+          __syncwarp();
+        }
+        act_forward(v[0], p.act);
+        act_forward(v[1], p.act);
+        if (p.residual) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) *staged(stg, k, lane) = res[k];
+          __syncwarp();
+          add_block(v, stg_at, lane);
+          __syncwarp();
+          load_block(res, p.residual, p.cols, row0 + 64, x.row_end, col0, lane);
+        }
+        put_block(v, stg_at, lane);
+        __syncwarp();
+        store_block(stg, p.out, p.cols, row0, x.row_end, col0, lane);
+        __syncwarp();
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (rank == 0)
+          mbar_arrive(tempty_bar(acc));
+        else
+          mbar_arrive_cluster(tempty_bar(acc), 0);
+      }
+      ++it;
+    }
+  }
+
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // the leader's MMAs into both TMEMs are complete
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc<2>(tmem_base, C::TMEM_COLS);
+}
+
+// ===========================================================================
+// outer_kernel
+// ===========================================================================
+// The weights' gradient dW[k, n] = sum over rows of X[row, k] dY[row, n], for
+// all rows or per group.  A cluster of two CTAs computes 256 x 256 tiles of
+// dW; CTA r holds rows k [128 r, 128 r + 128) and columns n
+// [128 r, 128 r + 128) of the operands, both MN-major as they are stored, and
+// owns its half's accumulator rows.  Persistent, like rows_kernel; the tiles
+// of the last wave are halved in n where that fills the pairs.  Warps: 0 TMA
+// producer, 1 MMA issuer (leader only), 2..9 epilogue (two warps per TMEM lane
+// quadrant, each half of the tile's 64-column slices), 10 (grouped only)
+// clears the rows behind a group's end.
+//
+// That is needed because the contraction runs over a group's rows, whose count
+// is any number: the last k-block also loads rows of the next group, or rows
+// behind the last one, whose values (NaN among them) must not count.  An
+// instruction takes 16 rows, so those that hold no row of the group are not
+// issued, and the rest of the last one's 16 rows, whole 128-byte lines of both
+// operands, is zeroed.  Such a block's loads complete on a barrier of the
+// CTA's own; warp 10 zeroes the lines and, once both CTAs have, releases the
+// block to the MMA thread.
+template <bool GROUPED_>
+struct OuterCfg {
+  static constexpr bool GROUPED = GROUPED_;
+  static constexpr int STAGES = 6;
+  static constexpr int BM = 128;  // rows (k) and columns (n) per CTA
+  static constexpr int BK = 64, CHUNK = 64, UMMA_K = 16;
+  static constexpr int CHUNK_BYTES = BK * 128;  // 64 values by 64 rows
+  static constexpr int A_BYTES = BM * 128;
+  static constexpr int STAGE_BYTES = 2 * A_BYTES;
+  static constexpr int TMEM_COLS = 512;
+  static constexpr int EPI_WARPS = 8;
+  static constexpr int THREADS = 32 * (2 + EPI_WARPS + (GROUPED ? 1 : 0));
+  static constexpr int RASTER = 8;  // tile rows walked column by column
+  static constexpr int STG_OFF = STAGES * STAGE_BYTES;
+  static constexpr int BAR_OFF = STG_OFF + EPI_WARPS * 2048;
+  static constexpr int NBARS = 2 * STAGES + 5 + (GROUPED ? 2 * STAGES : 0);
+  static constexpr int TAB_OFF = BAR_OFF + NBARS * 8 + 16;
+  static constexpr int TAB_BYTES = GROUPED ? (kMaxGroups + 1) * 4 : 0;
+  static constexpr int SMEM_BYTES = 1024 + TAB_OFF + TAB_BYTES;
+  // without the N field, which is the tile's
+  static constexpr u32 IDESC = make_idesc(1u, 1u, true, true, 256, 0);
+  static_assert(SMEM_BYTES <= 232448, "shared memory budget exceeded");
+};
+
+struct OuterTile {
+  int m0, n0;     // first row k and column n of the tile
+  int chunks;     // 64-column chunks per CTA: 2, or 1 for half a tile
+  int grp;        // group, 0 when dense
+  int r0;         // first row of the contraction
+  int nkb, tail;  // k-blocks; valid rows of the last one, 0 when whole (or dense)
+};
+
+template <class C>
+struct OuterWalk {
+  const GemmArgs &g;
+  const int *tab_off;
+  int i, step, whole, items, ntm, ntn;
+  bool halves;
+
+  __device__ __forceinline__ OuterWalk(const GemmArgs &g_, const int *o)
+      : g(g_), tab_off(o), i(blockIdx.x / 2), step(gridDim.x / 2) {
+    ntm = (g.GM + 255) / 256;
+    ntn = (g.GN + 255) / 256;
+    const int total = ntm * ntn * (C::GROUPED ? g.groups : 1);
+    const int rest = total % step;
+    whole = total - rest;
+    halves = 2 * rest <= step;
+    items = whole + rest * (halves ? 2 : 1);
+  }
+
+  __device__ __forceinline__ bool next(OuterTile &x) {
+    for (; i < items; i += step) {
+      int t = i, part = 0;
+      x.chunks = 2;
+      if (i >= whole && halves) {
+        t = whole + (i - whole) / 2;
+        part = (i - whole) & 1;
+        x.chunks = 1;
+      }
+      x.grp = C::GROUPED ? t / (ntm * ntn) : 0;
+      const int local = t - x.grp * ntm * ntn, per = C::RASTER * ntn;
+      const int q = local / per, r = local - q * per;
+      const int band = min(ntm - q * C::RASTER, C::RASTER);
+      x.m0 = (q * C::RASTER + r % band) * 256;
+      x.n0 = r / band * 256 + part * 128;
+      if (x.n0 >= g.GN) continue;  // the second half of a tile that has only one
+      const int len = C::GROUPED ? tab_off[x.grp + 1] - tab_off[x.grp] : g.GK;
+      x.r0 = C::GROUPED ? tab_off[x.grp] : 0;
+      x.nkb = (len + C::BK - 1) / C::BK;
+      x.tail = C::GROUPED ? len % C::BK : 0;  // dense: TMA fills rows past the end with zeros
+      i += step;
+      return true;
+    }
+    return false;
+  }
+};
+
+template <class C>
+__global__ void __launch_bounds__(C::THREADS, 1)
+    outer_kernel(const __grid_constant__ TensorMap tmap_x, const __grid_constant__ TensorMap tmap_y,
+                 const GemmArgs g) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   const u32 raw = smem_u32(smem_raw);
   const u32 base = (raw + 1023u) & ~1023u;
@@ -418,7 +803,6 @@ __global__ void __launch_bounds__(C::THREADS, 1)
   u32 *tmem_slot = reinterpret_cast<u32 *>(smem + C::BAR_OFF + C::NBARS * 8);
   volatile u32 *abort_flag = tmem_slot + 1;
   int *tab_off = reinterpret_cast<int *>(smem + C::TAB_OFF);
-  int *tab_tile = C::MODE == GROUP_ROWS ? tab_off + kMaxGroups + 1 : nullptr;
   u32 *status = g.epi.status;
 
   const int warp = threadIdx.x / 32;
@@ -429,7 +813,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     for (int s = 0; s < C::STAGES; ++s) {
       mbar_init(full_bar(s), 1);
       mbar_init(empty_bar(s), 1);
-      if (C::MODE == GROUP_K) {
+      if (C::GROUPED) {
         mbar_init(tail_bar(s), 1);
         mbar_init(fixed_bar(s), 1);
       }
@@ -441,16 +825,16 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     mbar_init(drain_bar, 1);
     *abort_flag = 0;
     fence_mbar_init();
-    tma_prefetch_desc(&tmap_a);
-    tma_prefetch_desc(&tmap_b);
+    tma_prefetch_desc(&tmap_x);
+    tma_prefetch_desc(&tmap_y);
   }
   if (warp == 1) {
     tmem_alloc<2>(smem_u32(tmem_slot), C::TMEM_COLS);
     tmem_relinquish<2>();
   }
-  if (C::MODE != DENSE && warp == 2) {
+  if (C::GROUPED && warp == 2) {
     pdl_wait();  // the offsets may come from the previous kernel of the stream
-    scan_groups(g.offsets, g.groups, g.rows, 256, tab_off, tab_tile, blockIdx.x == 0 ? status : nullptr);
+    scan_groups(g.offsets, g.groups, g.rows, 256, tab_off, nullptr, blockIdx.x == 0 ? status : nullptr);
   }
   tc_fence_before();
   __syncthreads();
@@ -463,43 +847,32 @@ __global__ void __launch_bounds__(C::THREADS, 1)
   if (warp == 0) {
     // ------------------------------------------------ TMA producer (both CTAs)
     if (lane == 0) {
-      Walk<C> walk(g, tab_off, tab_tile);
-      Tile x;
+      OuterWalk<C> walk(g, tab_off);
+      OuterTile x;
       int s = 0;
       u32 ph = 0;
       while (!*abort_flag && walk.next(x)) {
-        const int am = x.m0 + rank * C::BM, bn = x.n0 + rank * C::BNH;
+        const int m = x.m0 + rank * C::BM, n = x.n0 + rank * x.chunks * C::CHUNK;
+        const u32 bytes = C::A_BYTES + x.chunks * C::CHUNK_BYTES;
         for (int kb = 0; kb < x.nkb; ++kb) {
           if (!mbar_wait(empty_bar(s), ph ^ 1u, status, 0x41)) {
             *abort_flag = 1;
             break;
           }
-          const u32 sa = base + s * C::STAGE_BYTES, sb = sa + C::A_BYTES;
+          const u32 sx = base + s * C::STAGE_BYTES, sy = sx + C::A_BYTES;
           u32 fb;
-          if (C::MODE == GROUP_K && x.tail && kb == x.nkb - 1) {
-            fb = tail_bar(s);
-            mbar_arrive_expect_tx(fb, C::STAGE_BYTES);
-            fb = mapa_cluster(fb, rank);
+          if (C::GROUPED && x.tail && kb == x.nkb - 1) {
+            mbar_arrive_expect_tx(tail_bar(s), bytes);
+            fb = mapa_cluster(tail_bar(s), rank);
           } else {
-            if (rank == 0) mbar_arrive_expect_tx(full_bar(s), 2 * C::STAGE_BYTES);
+            if (rank == 0) mbar_arrive_expect_tx(full_bar(s), 2 * bytes);
             fb = mapa_cluster(full_bar(s), 0);
           }
-          const int k = x.k0 + kb * C::BK;
-          if (C::A_MN) {
-#pragma unroll
-            for (int c = 0; c < C::BM / C::CHUNK; ++c)
-              tma_load_3d_pair(sa + c * C::BK * 128, &tmap_a, fb, am + c * C::CHUNK, k, 0);
-          } else {
-            tma_load_3d_pair(sa, &tmap_a, fb, k, am, 0);
-          }
-          const int z = C::MODE == GROUP_ROWS ? x.grp : 0;
-          if (C::B_MN) {
-#pragma unroll
-            for (int c = 0; c < C::BNH / C::CHUNK; ++c)
-              tma_load_3d_pair(sb + c * C::BK * 128, &tmap_b, fb, bn + c * C::CHUNK, k, z);
-          } else {
-            tma_load_3d_pair(sb, &tmap_b, fb, k, bn, z);
-          }
+          const int row = x.r0 + kb * C::BK;
+          tma_load_3d_pair(sx, &tmap_x, fb, m, row, 0);
+          tma_load_3d_pair(sx + C::CHUNK_BYTES, &tmap_x, fb, m + C::CHUNK, row, 0);
+          tma_load_3d_pair(sy, &tmap_y, fb, n, row, 0);
+          if (x.chunks == 2) tma_load_3d_pair(sy + C::CHUNK_BYTES, &tmap_y, fb, n + C::CHUNK, row, 0);
           if (++s == C::STAGES) {
             s = 0;
             ph ^= 1u;
@@ -519,47 +892,51 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     // ------------------------------------------------ MMA issuer (leader CTA)
     // all of it in lane 0: a warp-wide step per k-block idles the tensor pipe
     if (rank == 0 && lane == 0) {
-      Walk<C> walk(g, tab_off, tab_tile);
-      Tile x;
+      OuterWalk<C> walk(g, tab_off);
+      OuterTile x;
       int s = 0, it = 0;
       u32 ph = 0;
       while (!*abort_flag && walk.next(x)) {
         if (x.nkb == 0) continue;  // an empty group's gradient: the epilogue writes zeros
         const int acc = it & 1;
-        const u32 d_tmem = tmem_base + acc * C::BN;
+        const u32 d_tmem = tmem_base + acc * (C::TMEM_COLS / 2);
         if (!mbar_wait(tempty_bar(acc), ((it >> 1) & 1) ^ 1u, status, 0x43)) {
           *abort_flag = 1;
           break;
         }
         tc_fence_after();
         bool ok = true;
-        for (int kb = 0; kb < x.nkb; ++kb) {
-          if (!mbar_wait(full_bar(s), ph, status, 0x44)) {
-            *abort_flag = 1;
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const u32 sa = base + s * C::STAGE_BYTES, sb = sa + C::A_BYTES;
+        auto run = [&](auto chunks) {
+          constexpr u32 idesc = C::IDESC | (decltype(chunks)::value * 128 >> 3) << 17;
+          for (int kb = 0; kb < x.nkb; ++kb) {
+            if (!mbar_wait(full_bar(s), ph, status, 0x44)) {
+              *abort_flag = 1;
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const u32 sx = base + s * C::STAGE_BYTES, sy = sx + C::A_BYTES;
+            const int steps = C::GROUPED && x.tail && kb == x.nkb - 1 ? (x.tail + C::UMMA_K - 1) / C::UMMA_K
+                                                                      : C::BK / C::UMMA_K;
 #pragma unroll
-          for (int k = 0; k < C::BK / C::UMMA_K; ++k) {
-            const u64 ad = C::A_MN ? smem_desc_sw128(sa + k * C::UMMA_K * 128, C::BK * 128, 1024)
-                                   : smem_desc_sw128(sa + k * 32, 16, 1024);
-            const u64 bd = C::B_MN ? smem_desc_sw128(sb + k * C::UMMA_K * 128, C::BK * 128, 1024)
-                                   : smem_desc_sw128(sb + k * 32, 16, 1024);
-            const u32 accum = (kb > 0 || k > 0) ? 1u : 0u;
-            if (C::KIND == KIND_BF16)
-              mma2_f16_ss(d_tmem, ad, bd, C::IDESC, accum);
-            else
-              mma2_f8f6f4_ss(d_tmem, ad, bd, C::IDESC, accum);
+            for (int k = 0; k < C::BK / C::UMMA_K; ++k) {
+              if (C::GROUPED && k >= steps) break;
+              const u64 ad = smem_desc_sw128(sx + k * C::UMMA_K * 128, C::CHUNK_BYTES, 1024);
+              const u64 bd = smem_desc_sw128(sy + k * C::UMMA_K * 128, C::CHUNK_BYTES, 1024);
+              mma2_f16_ss(d_tmem, ad, bd, idesc, (kb > 0 || k > 0) ? 1u : 0u);
+            }
+            tc_commit2(mapa_cluster(empty_bar(s), 0));
+            tc_commit2(mapa_cluster(empty_bar(s), 1));
+            if (++s == C::STAGES) {
+              s = 0;
+              ph ^= 1u;
+            }
           }
-          tc_commit2(mapa_cluster(empty_bar(s), 0));
-          tc_commit2(mapa_cluster(empty_bar(s), 1));
-          if (++s == C::STAGES) {
-            s = 0;
-            ph ^= 1u;
-          }
-        }
+        };
+        if (x.chunks == 2)
+          run(Const<2>());
+        else
+          run(Const<1>());
         if (!ok || *abort_flag) break;
         tc_commit2(mapa_cluster(tfull_bar(acc), 0));
         tc_commit2(mapa_cluster(tfull_bar(acc), 1));
@@ -569,10 +946,10 @@ __global__ void __launch_bounds__(C::THREADS, 1)
       mbar_wait(drain_bar, 0, status, 0x45);
     }
     __syncwarp();
-  } else if (C::MODE == GROUP_K && warp == 2 + C::EPI_WARPS) {
+  } else if (C::GROUPED && warp == 2 + C::EPI_WARPS) {
     // ------------------------------------------------ rows behind a group's end
-    Walk<C> walk(g, tab_off, tab_tile);
-    Tile x;
+    OuterWalk<C> walk(g, tab_off);
+    OuterTile x;
     int s = 0;
     u32 uses = 0;  // bit s: parity of the next use of stage s's tail barriers
     while (!*abort_flag && walk.next(x)) {
@@ -587,13 +964,12 @@ __global__ void __launch_bounds__(C::THREADS, 1)
           *abort_flag = 1;
           break;
         }
-        constexpr int LINES = C::STAGE_BYTES / 128 / C::BK;  // 128-byte columns of A and B
         unsigned char *st = smem + s * C::STAGE_BYTES;
-        for (int i = x.tail * 8 + lane; i < C::BK * 8; i += 32) {
-#pragma unroll
-          for (int c = 0; c < LINES; ++c)
-            *reinterpret_cast<uint4 *>(st + c * C::BK * 128 + i * 16) = make_uint4(0, 0, 0, 0);
-        }
+        const int end = (x.tail + C::UMMA_K - 1) / C::UMMA_K * C::UMMA_K;  // rows that an instruction reads
+        const int lines = 2 + x.chunks;                                    // 128-byte columns of both operands
+        for (int i = x.tail * 8 + lane; i < end * 8; i += 32)
+          for (int c = 0; c < lines; ++c)
+            *reinterpret_cast<uint4 *>(st + c * C::CHUNK_BYTES + i * 16) = make_uint4(0, 0, 0, 0);
         fence_proxy_async_smem();  // the MMA reads through the async proxy
         __syncwarp();
         if (lane == 0) {
@@ -612,20 +988,14 @@ __global__ void __launch_bounds__(C::THREADS, 1)
   } else {
     // ------------------------------------------------ epilogue (both CTAs)
     const int q = warp & 3;            // TMEM lane quadrant this warp may access
-    const int half = (warp - 2) >> 2;  // which half of the tile's columns
-    constexpr int SLICES = C::BN / 128;
-    unsigned char *stg = smem + C::STG_OFF + (warp - 2) * 4096;
-    Walk<C> walk(g, tab_off, tab_tile);
-    Tile x;
+    const int half = (warp - 2) >> 2;  // takes 32-column slices half, half + 2, ...
+    unsigned char *stg = smem + C::STG_OFF + (warp - 2) * 2048;
+    OuterWalk<C> walk(g, tab_off);
+    OuterTile x;
     int it = 0;
     while (!*abort_flag && walk.next(x)) {
-      Epilogue p = g.epi;
-      if (C::MODE == GROUP_K) p.out += static_cast<long long>(x.grp) * g.GM * g.GN;
-      const float alpha = p.group_scale ? p.alpha * __ldg(p.group_scale + x.grp) : p.alpha;
+      unsigned short *out = g.epi.out + static_cast<long long>(x.grp) * g.GM * g.GN;
       const int row0 = x.m0 + rank * C::BM + q * 32;
-      const int c0 = half * SLICES * 64;
-      uint4 res[8];
-      if (p.residual) load_residual(res, p, row0, x.row_end, x.n0 + c0, lane);
       const int acc = it & 1;
       if (x.nkb) {
         bool ok = true;
@@ -636,14 +1006,33 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         }
         tc_fence_after();
       }
-      const u32 t_row = tmem_base + (static_cast<u32>(q * 32) << 16) + acc * C::BN + c0;
+      const u32 t_row = tmem_base + (static_cast<u32>(q * 32) << 16) + acc * (C::TMEM_COLS / 2);
+      // thread = row: a row's 32 columns leave through this warp's staging
+      // block (rows of 64 bytes, chunks as in rows_kernel's)
 #pragma unroll 1
-      for (int i = 0; i < SLICES; ++i) {
-        if (row0 < x.row_end && x.n0 + c0 + 64 * i < p.cols)
-          epilogue_slice(p, t_row + 64 * i, x.nkb == 0, alpha, row0, x.row_end, x.n0 + c0 + 64 * i, res,
-                         stg, lane);
-        if (p.residual && i + 1 < SLICES)
-          load_residual(res, p, row0, x.row_end, x.n0 + c0 + 64 * (i + 1), lane);
+      for (int i = half; i < 4 * x.chunks; i += 2) {
+        const int col0 = x.n0 + 32 * i;
+        if (row0 >= g.GM || col0 >= g.GN) break;
+        u32 r[32];
+        if (x.nkb) {
+          tmem_ld_32x32b_x32(t_row + 32 * i, r);
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) r[j] = 0u;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          u32 w[4];
+#pragma unroll
+          for (int h = 0; h < 4; ++h)
+            w[h] = pack_bf16x2(__uint_as_float(r[8 * j + 2 * h]), __uint_as_float(r[8 * j + 2 * h + 1]));
+          *reinterpret_cast<uint4 *>(stg + lane * 64 + ((j ^ ((lane >> 1) & 3)) * 16)) =
+              make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        __syncwarp();
+        store_block(stg, out, g.GN, row0, g.GM, col0, lane);
+        __syncwarp();
       }
       if (x.nkb) {
         tc_fence_before();
@@ -928,27 +1317,27 @@ __global__ void __launch_bounds__(C::THREADS)
 // slope_kernel
 // ===========================================================================
 // dpre = dout * act'(preact), and/or the column sums of dpre (before its
-// rounding) over all rows.  A cluster of CTAs owns 128 columns: 16 threads
-// cover a row's 256 bytes, each CTA every R-th block of 16 rows; a thread's
-// eight column sums meet in shared memory and then over the cluster, in a
-// fixed order.
+// rounding) over all rows.  A block owns 128 columns and every `split`-th
+// block of 16 rows: 16 threads cover a row's 256 bytes.  For the sums the
+// `split` blocks of a column stripe are a cluster: a thread's eight column
+// sums meet in shared memory and then over the cluster, in a fixed order.
 struct SlopeArgs {
   const unsigned short *dout, *preact;
   unsigned short *dpre;
   float *dbias;
-  int rows, cols, act;
+  int rows, cols, act, split;
   const int *offsets;  // grouped: rows [offsets[0], offsets[groups]) only
   int groups;
 };
 
-__global__ void __launch_bounds__(256) slope_kernel(const SlopeArgs a) {
-  __shared__ float part[16][128];
-  __shared__ float sum[128];
+constexpr int kSlopeThreads = 256, kSlopeRows = kSlopeThreads / 16;
+
+__global__ void __launch_bounds__(kSlopeThreads, 4) slope_kernel(const SlopeArgs a) {
+  __shared__ float part[kSlopeThreads / 32][128];
   __shared__ int last;
   const int tid = threadIdx.x;
-  const int R = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
-  const int col = blockIdx.x / R * 128 + (tid & 15) * 8;
-  const bool in = col < a.cols;
+  const int stripe = blockIdx.x / a.split, rank = blockIdx.x - stripe * a.split;
+  const int col = stripe * 128 + (tid & 15) * 8;
   pdl_launch_dependents();
   pdl_wait();
   int lo = 0, hi = a.rows;
@@ -956,68 +1345,72 @@ __global__ void __launch_bounds__(256) slope_kernel(const SlopeArgs a) {
     // the last group ends at the largest clamped offset
     if (tid == 0) last = 0;
     __syncthreads();
-    for (int i = tid; i <= a.groups; i += 256) atomicMax(&last, min(a.offsets[i], a.rows));
+    for (int i = tid; i <= a.groups; i += kSlopeThreads) atomicMax(&last, min(a.offsets[i], a.rows));
     __syncthreads();
     lo = max(0, min(a.offsets[0], a.rows));
     hi = last;
   }
   float acc[8] = {};
-  if (in) {
-    constexpr int U = 4;  // rows in flight per thread
-    for (int row = lo + rank * 16 + (tid >> 4); row < hi; row += U * 16 * R) {
+  if (col < a.cols) {
+    constexpr int U = 2;  // rows in flight per thread
+    const int stride = kSlopeRows * a.split;
+    for (int row = lo + rank * kSlopeRows + (tid >> 4); row < hi; row += U * stride) {
       uint4 d[U], z[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int r = row + u * 16 * R;
+        const int r = row + u * stride;
         const long long off = static_cast<long long>(r) * a.cols + col;
         d[u] = z[u] = make_uint4(0, 0, 0, 0);
         if (r < hi) {
-          d[u] = __ldg(reinterpret_cast<const uint4 *>(a.dout + off));
-          if (a.preact) z[u] = __ldg(reinterpret_cast<const uint4 *>(a.preact + off));
+          d[u] = __ldcs(reinterpret_cast<const uint4 *>(a.dout + off));
+          if (a.preact) z[u] = __ldcs(reinterpret_cast<const uint4 *>(a.preact + off));
         }
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int r = row + u * 16 * R;
+        const int r = row + u * stride;
         if (r >= hi) break;
         const u32 dw[4] = {d[u].x, d[u].y, d[u].z, d[u].w}, zw[4] = {z[u].x, z[u].y, z[u].z, z[u].w};
-        u32 o[4];
+        float x[8], y[8];
 #pragma unroll
         for (int h = 0; h < 4; ++h) {
-          float x = bf16_lo(dw[h]), y = bf16_hi(dw[h]);
-          if (a.preact) {
-            x *= act_slope(bf16_lo(zw[h]), a.act);
-            y *= act_slope(bf16_hi(zw[h]), a.act);
-          }
-          acc[2 * h] += x;
-          acc[2 * h + 1] += y;
-          o[h] = pack_bf16x2(x, y);
+          x[2 * h] = bf16_lo(dw[h]);
+          x[2 * h + 1] = bf16_hi(dw[h]);
+          y[2 * h] = bf16_lo(zw[h]);
+          y[2 * h + 1] = bf16_hi(zw[h]);
         }
+        if (a.preact) act_backward(x, y, a.act);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[i] += x[i];
         if (a.dpre)
-          st_global_v4(a.dpre + static_cast<long long>(r) * a.cols + col, o[0], o[1], o[2], o[3]);
+          st_global_v4(a.dpre + static_cast<long long>(r) * a.cols + col, pack_bf16x2(x[0], x[1]),
+                       pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
       }
     }
   }
   if (!a.dbias) return;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) part[tid >> 4][(tid & 15) * 8 + i] = acc[i];
+  for (int i = 0; i < 8; ++i) {
+    acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], 16);  // the warp's two rows
+    if ((tid & 31) < 16) part[tid >> 5][(tid & 15) * 8 + i] = acc[i];
+  }
   __syncthreads();
   if (tid < 128) {
     float s = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s += part[i][tid];
-    sum[tid] = s;
+    for (int i = 0; i < kSlopeThreads / 32; ++i) s += part[i][tid];
+    part[0][tid] = s;
   }
   __syncthreads();
-  if (R > 1) cluster_sync();
+  if (a.split > 1) cluster_sync();
   if (rank == 0 && tid < 128) {
-    float s = sum[tid];
-    for (int c = 1; c < R; ++c) s += ld_cluster_f32(mapa_cluster(smem_u32(&sum[tid]), c));
-    const int n = blockIdx.x / R * 128 + tid;
+    float s = part[0][tid];
+    for (int c = 1; c < a.split; ++c) s += ld_cluster_f32(mapa_cluster(smem_u32(&part[0][tid]), c));
+    const int n = stripe * 128 + tid;
     if (n < a.cols) a.dbias[n] = s;
   }
   __syncwarp();
-  if (R > 1) cluster_sync();
+  if (a.split > 1) cluster_sync();
 }
 
 }  // namespace lin

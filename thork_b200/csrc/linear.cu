@@ -60,18 +60,6 @@ int launch(void (*kern)(KArgs...), unsigned grid, int threads, int smem, int clu
 }
 
 template <class C>
-int run_pair(const TensorMap &ta, const TensorMap &tb, const GemmArgs &g, long long tiles,
-             cudaStream_t s, const char *what) {
-  static std::atomic<uint64_t> done{0};
-  int rc, sms;
-  auto kern = pair_kernel<C>;
-  if ((rc = allow_smem(reinterpret_cast<const void *>(kern), C::SMEM_BYTES, done))) return rc;
-  if ((rc = thork_sm_count(&sms))) return rc;
-  const int pairs = static_cast<int>(tiles < sms / 2 ? tiles : sms / 2);
-  return launch(kern, 2 * pairs, C::THREADS, C::SMEM_BYTES, 2, s, what, ta, tb, g);
-}
-
-template <class C>
 int run_swap(const TensorMap &tw, const TensorMap &tx, const GemmArgs &g, long long items, int split,
              cudaStream_t s, const char *what) {
   static std::atomic<uint64_t> done{0};
@@ -141,23 +129,28 @@ int swap_product(const Product &p, const GemmArgs &g, cudaStream_t s, const char
   return run_swap<C>(tw, tx, g, rt * ntn, static_cast<int>(split), s, what);
 }
 
-template <int KIND, int BN, int STAGES, bool W_MN, int MODE>
-int pair_product(const Product &p, const GemmArgs &g, cudaStream_t s, const char *what) {
-  using C = PairCfg<KIND, BN, STAGES, false, W_MN, MODE>;
-  int rc;
-  alignas(64) TensorMap ta, tb;
-  if ((rc = map_x<KIND>(ta, p, C::BM))) return rc;
-  if ((rc = map_w<KIND, W_MN>(tb, p, C::BNH))) return rc;
-  long long rt = (p.rows + 255) / 256;
-  if (MODE == GROUP_ROWS) rt += p.groups < p.rows ? p.groups : p.rows;
-  return run_pair<C>(ta, tb, g, rt * ((p.n + BN - 1) / BN), s, what);
+template <int KIND, bool W_MN, bool GROUPED>
+int rows_product(const Product &p, const GemmArgs &g, cudaStream_t s, const char *what) {
+  using C = RowsCfg<KIND, W_MN, GROUPED>;
+  static std::atomic<uint64_t> done{0};
+  int rc, sms;
+  alignas(64) TensorMap tw, tx, txu;
+  if ((rc = map_w<KIND, W_MN>(tw, p, C::BNC))) return rc;
+  if ((rc = map_x<KIND>(tx, p, C::MAX_UNITS * C::BOX_ROWS))) return rc;
+  if ((rc = map_x<KIND>(txu, p, C::BOX_ROWS))) return rc;
+  auto kern = rows_kernel<C>;
+  if ((rc = allow_smem(reinterpret_cast<const void *>(kern), C::SMEM_BYTES, done))) return rc;
+  if ((rc = thork_sm_count(&sms))) return rc;
+  // one pair per unit of 64 rows and 256 columns at most
+  long long units = (static_cast<long long>(p.rows) + C::UNIT - 1) / C::UNIT;
+  if (GROUPED) units += p.groups < p.rows ? p.groups : p.rows;
+  const long long most = units * ((p.n + 2 * C::BNC - 1) / (2 * C::BNC));
+  const int pairs = static_cast<int>(most < sms / 2 ? most : sms / 2);
+  return launch(kern, 2 * pairs, C::THREADS, C::SMEM_BYTES, 2, s, what, tw, tx, txu, g);
 }
 
 template <int KIND, bool W_MN, bool GROUPED>
 int product(const Product &p, const GemmArgs &g, cudaStream_t s, const char *what) {
-  constexpr int MODE = GROUPED ? GROUP_ROWS : DENSE;
-  int rc, sms;
-  if ((rc = thork_sm_count(&sms))) return rc;
   // rows that a tile can expect: of the whole product, or of one group
   const long long rows = GROUPED ? (static_cast<long long>(p.rows) + p.groups - 1) / p.groups : p.rows;
   constexpr int G = GROUPED ? 1 : 0;  // the group table takes one stage's room
@@ -165,38 +158,41 @@ int product(const Product &p, const GemmArgs &g, cudaStream_t s, const char *wha
   if (rows <= 32) return swap_product<KIND, 32, 5, W_MN, GROUPED>(p, g, s, what);
   if (rows <= 64) return swap_product<KIND, 64, 4, W_MN, GROUPED>(p, g, s, what);
   if (rows <= 128) return swap_product<KIND, 128, 3, W_MN, GROUPED>(p, g, s, what);
-  if constexpr (KIND == KIND_BF16) {
-    const long long tiles = ((p.rows + 255) / 256) * static_cast<long long>((p.n + 255) / 256);
-    if (tiles < sms / 2) return pair_product<KIND, 128, 8 - 2 * G, W_MN, MODE>(p, g, s, what);
-  }
-  return pair_product<KIND, 256, 6 - G, W_MN, MODE>(p, g, s, what);
+  return rows_product<KIND, W_MN, GROUPED>(p, g, s, what);
 }
 
 // dW[k, n] = sum over rows X[m, k] dY[m, n], of each group's rows when grouped.
-template <int BN, int STAGES, int MODE>
-int weight_gradient(const void *x, const void *dy, int rows, int n, int k, int groups, const GemmArgs &g,
+template <bool GROUPED>
+int weight_gradient(const void *x, const void *dy, int rows, int n, int k, const GemmArgs &g,
                     cudaStream_t s, const char *what) {
-  using C = PairCfg<KIND_BF16, BN, STAGES, true, true, MODE>;
-  int rc;
-  alignas(64) TensorMap ta, tb;
-  if ((rc = thork_encode_tmap_3d(&ta, THORK_DT_BF16, x, k, rows, 1, 64, 64))) return rc;
-  if ((rc = thork_encode_tmap_3d(&tb, THORK_DT_BF16, dy, n, rows, 1, 64, 64))) return rc;
-  const long long tiles = ((k + 255) / 256) * static_cast<long long>((n + BN - 1) / BN) * (groups ? groups : 1);
-  return run_pair<C>(ta, tb, g, tiles, s, what);
+  using C = OuterCfg<GROUPED>;
+  static std::atomic<uint64_t> done{0};
+  int rc, sms;
+  alignas(64) TensorMap tx, ty;
+  if ((rc = thork_encode_tmap_3d(&tx, THORK_DT_BF16, x, k, rows, 1, C::CHUNK, C::BK))) return rc;
+  if ((rc = thork_encode_tmap_3d(&ty, THORK_DT_BF16, dy, n, rows, 1, C::CHUNK, C::BK))) return rc;
+  auto kern = outer_kernel<C>;
+  if ((rc = allow_smem(reinterpret_cast<const void *>(kern), C::SMEM_BYTES, done))) return rc;
+  if ((rc = thork_sm_count(&sms))) return rc;
+  // one pair per half of a tile at most
+  const long long most = 2ll * ((k + 255) / 256) * ((n + 255) / 256) * (GROUPED ? g.groups : 1);
+  const int pairs = static_cast<int>(most < sms / 2 ? most : sms / 2);
+  return launch(kern, 2 * pairs, C::THREADS, C::SMEM_BYTES, 2, s, what, tx, ty, g);
 }
 
-int slope(const SlopeArgs &a, cudaStream_t s, const char *what) {
+int slope(SlopeArgs a, cudaStream_t s, const char *what) {
   int rc, sms;
   if ((rc = thork_sm_count(&sms))) return rc;
   const long long stripes = (a.cols + 127) / 128;
-  // eight blocks of 256 threads per SM, at most one per 64 rows
-  long long split = 8ll * sms / stripes;
-  const long long most = (a.rows + 63) / 64;
+  // two waves of four blocks per SM, at most one per 32 rows; the column
+  // sums' blocks are a cluster, of at most eight
+  long long split = (8ll * sms + stripes - 1) / stripes;
+  const long long most = (a.rows + 31) / 32;
   if (split > most) split = most;
-  if (split > 8) split = 8;
-  if (split < 1) split = 1;
-  return launch(slope_kernel, static_cast<unsigned>(stripes * split), 256, 0, static_cast<int>(split), s,
-                what, a);
+  if (a.dbias && split > 8) split = 8;
+  a.split = static_cast<int>(split);
+  return launch(slope_kernel, static_cast<unsigned>(stripes * split), kSlopeThreads, 0, a.dbias ? a.split : 1, s, what,
+                a);
 }
 
 // ---------------------------------------------------------------- checks
@@ -319,7 +315,7 @@ int backward(void *da, void *db, float *dbias, const void *dout, const void *a, 
   if (bent || dbias) {
     const SlopeArgs sl = {static_cast<const unsigned short *>(dout),
                           static_cast<const unsigned short *>(preact), static_cast<unsigned short *>(dpre),
-                          dbias, rows, N, act, offsets, groups};
+                          dbias, rows, N, act, 1, offsets, groups};
     if ((rc = slope(sl, s, what))) return rc;
   }
   const void *dz = bent ? dpre : dout;
@@ -341,22 +337,14 @@ int backward(void *da, void *db, float *dbias, const void *dout, const void *a, 
     if (rc) return rc;
   }
   if (db) {
-    int sms;
-    if ((rc = thork_sm_count(&sms))) return rc;
     GemmArgs w = g;
     w.epi.out = static_cast<unsigned short *>(db);
     w.epi.cols = N;
     w.GM = K;
     w.GN = N;
     w.GK = rows;
-    const long long tiles = ((K + 255) / 256) * static_cast<long long>((N + 255) / 256) * (groups ? groups : 1);
-    const bool wide = tiles >= sms / 2;
-    if (groups)
-      rc = wide ? weight_gradient<256, 5, GROUP_K>(a, dz, rows, N, K, groups, w, s, what)
-                : weight_gradient<128, 6, GROUP_K>(a, dz, rows, N, K, groups, w, s, what);
-    else
-      rc = wide ? weight_gradient<256, 6, DENSE>(a, dz, rows, N, K, 0, w, s, what)
-                : weight_gradient<128, 8, DENSE>(a, dz, rows, N, K, 0, w, s, what);
+    rc = groups ? weight_gradient<true>(a, dz, rows, N, K, w, s, what)
+                : weight_gradient<false>(a, dz, rows, N, K, w, s, what);
     if (rc) return rc;
   }
   return THORK_OK;
