@@ -18,6 +18,7 @@ GROUPS = {
     "single rows": ([1, 0, 1, 1], 0, 0),
     "thin": ([0, 3, 16, 17, 0, 1, 40, 2], 0, 5),
     "first offset": ([7, 0, 9], 6, 3),
+    "sixteens": ([15, 16, 17, 31, 32, 33, 47, 48, 49, 80, 95], 0, 0),
     "tiles": ([64, 65, 128, 127, 63, 1], 0, 0),
     "wide": ([300, 0, 257, 256, 513], 0, 11),
     "skewed": ([1000, 2, 0, 130], 1, 1),

@@ -73,6 +73,14 @@ __device__ __forceinline__ void tma_load_3d_pair(u32 dst, const TensorMap *m, u3
       : "memory");
 }
 
+__device__ __forceinline__ void tma_store_3d(const TensorMap *m, u32 src, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+          reinterpret_cast<u64>(m)),
+      "r"(src), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
 __device__ __forceinline__ u32 cluster_nctarank() {
   u32 r;
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
@@ -267,6 +275,44 @@ struct RowsCfg {
   static_assert(SMEM_BYTES <= 232448, "shared memory budget exceeded");
 };
 
+// n / d for 0 <= n < 2^31 by a multiplication: every role of a persistent
+// kernel finds its tiles with a few of these, and a division instruction
+// sequence is long enough to show between short tiles.
+struct Divisor {
+  u32 d, m;
+  __device__ __forceinline__ explicit Divisor(int d_) : d(d_), m(0xFFFFFFFFu / static_cast<u32>(d_)) {}
+  // floor(n m / 2^32) is the quotient or one less, as n < 2^31
+  __device__ __forceinline__ int operator()(int n, int &rest) const {
+    u32 q = __umulhi(static_cast<u32>(n), m), r = static_cast<u32>(n) - q * d;
+    if (r >= d) {
+      ++q;
+      r -= d;
+    }
+    rest = static_cast<int>(r);
+    return static_cast<int>(q);
+  }
+};
+
+// Tile t of an ntm x ntn grid of tiles: bands of BAND tile rows are walked
+// column by column, so that the tiles in flight share operand panels in L2.
+template <int BAND>
+struct Raster {
+  Divisor band;  // tiles of a whole band
+  int ntn;
+  __device__ __forceinline__ explicit Raster(int ntn_) : band(BAND * ntn_), ntn(ntn_) {}
+  __device__ __forceinline__ void operator()(int t, int ntm, int &tm, int &tn) const {
+    int r;
+    const int q = band(t, r), first = q * BAND, rows = ntm - first;
+    if (rows >= BAND) {
+      tn = r / BAND;
+      tm = first + r % BAND;
+    } else {
+      tn = r / rows;
+      tm = first + r - tn * rows;
+    }
+  }
+};
+
 template <int N>
 struct Const {
   static constexpr int value = N;
@@ -285,10 +331,11 @@ struct RowWalk {
   const GemmArgs &g;
   const int *tab_off, *tab_tile;
   int i, step, whole, pieces, items, grp, ntn;
+  Raster<C::RASTER> raster;
 
   __device__ __forceinline__ RowWalk(const GemmArgs &g_, const int *o, const int *tl)
-      : g(g_), tab_off(o), tab_tile(tl), i(blockIdx.x / 2), step(gridDim.x / 2), grp(0) {
-    ntn = (g.GN + 2 * C::BNC - 1) / (2 * C::BNC);
+      : g(g_), tab_off(o), tab_tile(tl), i(blockIdx.x / 2), step(gridDim.x / 2), grp(0),
+        ntn((g_.GN + 2 * C::BNC - 1) / (2 * C::BNC)), raster(ntn) {
     const int total = (C::GROUPED ? tab_tile[g.groups] : row_tiles(g.GM)) * ntn;
     const int rest = total % step;
     whole = total - rest;
@@ -318,10 +365,8 @@ struct RowWalk {
       } else {
         ntm = row_tiles(rows);
       }
-      const int local = t - first * ntn, per = C::RASTER * ntn;
-      const int q = local / per, r = local - q * per;
-      const int band = min(ntm - q * C::RASTER, C::RASTER);
-      const int tn = r / band, tm = q * C::RASTER + r - tn * band;
+      int tm, tn;
+      raster(t - first * ntn, ntm, tm, tn);
       // the row tile's units, and of those the piece's
       const int units = min((rows - tm * (C::UNIT * C::MAX_UNITS) + C::UNIT - 1) / C::UNIT, C::MAX_UNITS);
       const int p0 = units * piece / parts, p1 = units * (piece + 1) / parts;
@@ -699,30 +744,40 @@ __global__ void __launch_bounds__(C::THREADS, 1)
 // quadrant, each half of the tile's 64-column slices), 10 (grouped only)
 // clears the rows behind a group's end.
 //
-// That is needed because the contraction runs over a group's rows, whose count
-// is any number: the last k-block also loads rows of the next group, or rows
-// behind the last one, whose values (NaN among them) must not count.  An
-// instruction takes 16 rows, so those that hold no row of the group are not
-// issued, and the rest of the last one's 16 rows, whole 128-byte lines of both
-// operands, is zeroed.  Such a block's loads complete on a barrier of the
-// CTA's own; warp 10 zeroes the lines and, once both CTAs have, releases the
-// block to the MMA thread.
+// The contraction runs over a group's rows, whose count is any number, and a
+// block of 64 rows that crosses the group's end also loads rows of the next
+// group, or rows behind the last one, whose values (NaN among them) must not
+// count.  An instruction takes 16 rows.  So the whole sixteens of the last
+// block are an ordinary block of which fewer instructions are issued, and the
+// last rows, fewer than 16, are a block of their own: its loads complete on a
+// barrier of the CTA's own, warp 10 zeroes the lines behind the group's end in
+// both operands and, once both CTAs have, releases it to the MMA thread.
+// These short blocks have two slots beside the ring, are fetched first and
+// used last, so that the round trip hides behind the tile's other blocks
+// (8 x [500, 4096]^T [500, 4096]: 158 us with the zeroing in the ring's order,
+// 128 without a remainder).
+//
+// A warp's 32 rows x 64 columns of the result leave through shared memory by
+// TMA, in whole 128-byte lines; it clips what lies outside dW.
 template <bool GROUPED_>
 struct OuterCfg {
   static constexpr bool GROUPED = GROUPED_;
-  static constexpr int STAGES = 6;
+  static constexpr int STAGES = GROUPED ? 5 : 6;
   static constexpr int BM = 128;  // rows (k) and columns (n) per CTA
   static constexpr int BK = 64, CHUNK = 64, UMMA_K = 16;
   static constexpr int CHUNK_BYTES = BK * 128;  // 64 values by 64 rows
   static constexpr int A_BYTES = BM * 128;
   static constexpr int STAGE_BYTES = 2 * A_BYTES;
+  static constexpr int SHORT_CHUNK = UMMA_K * 128;  // 64 values by 16 rows
+  static constexpr int SHORT_BYTES = 4 * SHORT_CHUNK;
   static constexpr int TMEM_COLS = 512;
   static constexpr int EPI_WARPS = 8;
   static constexpr int THREADS = 32 * (2 + EPI_WARPS + (GROUPED ? 1 : 0));
   static constexpr int RASTER = 8;  // tile rows walked column by column
-  static constexpr int STG_OFF = STAGES * STAGE_BYTES;
-  static constexpr int BAR_OFF = STG_OFF + EPI_WARPS * 2048;
-  static constexpr int NBARS = 2 * STAGES + 5 + (GROUPED ? 2 * STAGES : 0);
+  static constexpr int SHORT_OFF = STAGES * STAGE_BYTES;
+  static constexpr int STG_OFF = SHORT_OFF + (GROUPED ? 2 * SHORT_BYTES : 0);
+  static constexpr int BAR_OFF = STG_OFF + EPI_WARPS * 4096;
+  static constexpr int NBARS = 2 * STAGES + 5 + (GROUPED ? 8 : 0);
   static constexpr int TAB_OFF = BAR_OFF + NBARS * 8 + 16;
   static constexpr int TAB_BYTES = GROUPED ? (kMaxGroups + 1) * 4 : 0;
   static constexpr int SMEM_BYTES = 1024 + TAB_OFF + TAB_BYTES;
@@ -732,11 +787,12 @@ struct OuterCfg {
 };
 
 struct OuterTile {
-  int m0, n0;     // first row k and column n of the tile
-  int chunks;     // 64-column chunks per CTA: 2, or 1 for half a tile
-  int grp;        // group, 0 when dense
-  int r0;         // first row of the contraction
-  int nkb, tail;  // k-blocks; valid rows of the last one, 0 when whole (or dense)
+  int m0, n0;        // first row k and column n of the tile
+  int chunks;        // 64-column chunks per CTA: 2, or 1 for half a tile
+  int grp;           // group, 0 when dense
+  int r0;            // first row of the contraction
+  int blocks, last;  // 64-row blocks, and the instructions (16 rows) of the last one
+  int rest;          // rows behind them, fewer than 16 (grouped)
 };
 
 template <class C>
@@ -745,11 +801,12 @@ struct OuterWalk {
   const int *tab_off;
   int i, step, whole, items, ntm, ntn;
   bool halves;
+  Raster<C::RASTER> raster;
+  Divisor per_group;
 
   __device__ __forceinline__ OuterWalk(const GemmArgs &g_, const int *o)
-      : g(g_), tab_off(o), i(blockIdx.x / 2), step(gridDim.x / 2) {
-    ntm = (g.GM + 255) / 256;
-    ntn = (g.GN + 255) / 256;
+      : g(g_), tab_off(o), i(blockIdx.x / 2), step(gridDim.x / 2), ntm((g_.GM + 255) / 256),
+        ntn((g_.GN + 255) / 256), raster(ntn), per_group(ntm * ntn) {
     const int total = ntm * ntn * (C::GROUPED ? g.groups : 1);
     const int rest = total % step;
     whole = total - rest;
@@ -766,17 +823,19 @@ struct OuterWalk {
         part = (i - whole) & 1;
         x.chunks = 1;
       }
-      x.grp = C::GROUPED ? t / (ntm * ntn) : 0;
-      const int local = t - x.grp * ntm * ntn, per = C::RASTER * ntn;
-      const int q = local / per, r = local - q * per;
-      const int band = min(ntm - q * C::RASTER, C::RASTER);
-      x.m0 = (q * C::RASTER + r % band) * 256;
-      x.n0 = r / band * 256 + part * 128;
+      int local = t, tm, tn;
+      x.grp = C::GROUPED ? per_group(t, local) : 0;
+      raster(local, ntm, tm, tn);
+      x.m0 = tm * 256;
+      x.n0 = tn * 256 + part * 128;
       if (x.n0 >= g.GN) continue;  // the second half of a tile that has only one
       const int len = C::GROUPED ? tab_off[x.grp + 1] - tab_off[x.grp] : g.GK;
       x.r0 = C::GROUPED ? tab_off[x.grp] : 0;
-      x.nkb = (len + C::BK - 1) / C::BK;
-      x.tail = C::GROUPED ? len % C::BK : 0;  // dense: TMA fills rows past the end with zeros
+      // dense: TMA fills the rows behind the last with zeros
+      const int steps = C::GROUPED ? len / C::UMMA_K : (len + C::UMMA_K - 1) / C::UMMA_K;
+      x.rest = C::GROUPED ? len % C::UMMA_K : 0;
+      x.blocks = (steps + 3) / 4;
+      x.last = steps - 4 * (x.blocks - 1);
       i += step;
       return true;
     }
@@ -787,7 +846,8 @@ struct OuterWalk {
 template <class C>
 __global__ void __launch_bounds__(C::THREADS, 1)
     outer_kernel(const __grid_constant__ TensorMap tmap_x, const __grid_constant__ TensorMap tmap_y,
-                 const GemmArgs g) {
+                 const __grid_constant__ TensorMap tmap_x16, const __grid_constant__ TensorMap tmap_y16,
+                 const __grid_constant__ TensorMap tmap_out, const GemmArgs g) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   const u32 raw = smem_u32(smem_raw);
   const u32 base = (raw + 1023u) & ~1023u;
@@ -798,8 +858,12 @@ __global__ void __launch_bounds__(C::THREADS, 1)
   auto tfull_bar = [&](int a) { return bars + 8u * (2 * C::STAGES + a); };
   auto tempty_bar = [&](int a) { return bars + 8u * (2 * C::STAGES + 2 + a); };
   const u32 drain_bar = bars + 8u * (2 * C::STAGES + 4);
-  auto tail_bar = [&](int s) { return bars + 8u * (2 * C::STAGES + 5 + s); };   // this CTA's loads landed
-  auto fixed_bar = [&](int s) { return bars + 8u * (3 * C::STAGES + 5 + s); };  // leader: the peer has zeroed
+  // of the short blocks' two slots: this CTA's loads have landed; the peer has
+  // zeroed (leader's copy); both have (leader's); the MMA has read the slot
+  auto short_full = [&](int b) { return bars + 8u * (2 * C::STAGES + 5 + b); };
+  auto short_peer = [&](int b) { return bars + 8u * (2 * C::STAGES + 7 + b); };
+  auto short_ready = [&](int b) { return bars + 8u * (2 * C::STAGES + 9 + b); };
+  auto short_empty = [&](int b) { return bars + 8u * (2 * C::STAGES + 11 + b); };
   u32 *tmem_slot = reinterpret_cast<u32 *>(smem + C::BAR_OFF + C::NBARS * 8);
   volatile u32 *abort_flag = tmem_slot + 1;
   int *tab_off = reinterpret_cast<int *>(smem + C::TAB_OFF);
@@ -813,9 +877,13 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     for (int s = 0; s < C::STAGES; ++s) {
       mbar_init(full_bar(s), 1);
       mbar_init(empty_bar(s), 1);
-      if (C::GROUPED) {
-        mbar_init(tail_bar(s), 1);
-        mbar_init(fixed_bar(s), 1);
+    }
+    if (C::GROUPED) {
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(short_full(b), 1);
+        mbar_init(short_peer(b), 1);
+        mbar_init(short_ready(b), 1);
+        mbar_init(short_empty(b), 1);
       }
     }
     for (int a = 0; a < 2; ++a) {
@@ -849,25 +917,34 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     if (lane == 0) {
       OuterWalk<C> walk(g, tab_off);
       OuterTile x;
-      int s = 0;
+      int s = 0, shorts = 0;
       u32 ph = 0;
       while (!*abort_flag && walk.next(x)) {
         const int m = x.m0 + rank * C::BM, n = x.n0 + rank * x.chunks * C::CHUNK;
-        const u32 bytes = C::A_BYTES + x.chunks * C::CHUNK_BYTES;
-        for (int kb = 0; kb < x.nkb; ++kb) {
+        if (x.rest) {
+          const int b = shorts & 1, row = x.r0 + x.blocks * C::BK - (x.blocks ? (4 - x.last) * C::UMMA_K : 0);
+          if (!mbar_wait(short_empty(b), ((shorts >> 1) & 1) ^ 1u, status, 0x40)) {
+            *abort_flag = 1;
+            break;
+          }
+          ++shorts;
+          const u32 sx = base + C::SHORT_OFF + b * C::SHORT_BYTES, sy = sx + 2 * C::SHORT_CHUNK;
+          mbar_arrive_expect_tx(short_full(b), (2 + x.chunks) * C::SHORT_CHUNK);
+          const u32 fb = mapa_cluster(short_full(b), rank);
+          tma_load_3d_pair(sx, &tmap_x16, fb, m, row, 0);
+          tma_load_3d_pair(sx + C::SHORT_CHUNK, &tmap_x16, fb, m + C::CHUNK, row, 0);
+          tma_load_3d_pair(sy, &tmap_y16, fb, n, row, 0);
+          if (x.chunks == 2) tma_load_3d_pair(sy + C::SHORT_CHUNK, &tmap_y16, fb, n + C::CHUNK, row, 0);
+        }
+        const u32 bytes = 2 * (C::A_BYTES + x.chunks * C::CHUNK_BYTES);
+        for (int kb = 0; kb < x.blocks; ++kb) {
           if (!mbar_wait(empty_bar(s), ph ^ 1u, status, 0x41)) {
             *abort_flag = 1;
             break;
           }
           const u32 sx = base + s * C::STAGE_BYTES, sy = sx + C::A_BYTES;
-          u32 fb;
-          if (C::GROUPED && x.tail && kb == x.nkb - 1) {
-            mbar_arrive_expect_tx(tail_bar(s), bytes);
-            fb = mapa_cluster(tail_bar(s), rank);
-          } else {
-            if (rank == 0) mbar_arrive_expect_tx(full_bar(s), 2 * bytes);
-            fb = mapa_cluster(full_bar(s), 0);
-          }
+          if (rank == 0) mbar_arrive_expect_tx(full_bar(s), bytes);
+          const u32 fb = mapa_cluster(full_bar(s), 0);
           const int row = x.r0 + kb * C::BK;
           tma_load_3d_pair(sx, &tmap_x, fb, m, row, 0);
           tma_load_3d_pair(sx + C::CHUNK_BYTES, &tmap_x, fb, m + C::CHUNK, row, 0);
@@ -887,6 +964,8 @@ __global__ void __launch_bounds__(C::THREADS, 1)
           ph ^= 1u;
         }
       }
+      for (int i = 0; C::GROUPED && i < 2; ++i, ++shorts)
+        if (!mbar_wait(short_empty(shorts & 1), ((shorts >> 1) & 1) ^ 1u, status, 0x42)) break;
     }
   } else if (warp == 1) {
     // ------------------------------------------------ MMA issuer (leader CTA)
@@ -894,10 +973,10 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     if (rank == 0 && lane == 0) {
       OuterWalk<C> walk(g, tab_off);
       OuterTile x;
-      int s = 0, it = 0;
+      int s = 0, it = 0, shorts = 0;
       u32 ph = 0;
       while (!*abort_flag && walk.next(x)) {
-        if (x.nkb == 0) continue;  // an empty group's gradient: the epilogue writes zeros
+        if (x.blocks == 0 && x.rest == 0) continue;  // an empty group: the epilogue writes zeros
         const int acc = it & 1;
         const u32 d_tmem = tmem_base + acc * (C::TMEM_COLS / 2);
         if (!mbar_wait(tempty_bar(acc), ((it >> 1) & 1) ^ 1u, status, 0x43)) {
@@ -908,22 +987,24 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         bool ok = true;
         auto run = [&](auto chunks) {
           constexpr u32 idesc = C::IDESC | (decltype(chunks)::value * 128 >> 3) << 17;
-          for (int kb = 0; kb < x.nkb; ++kb) {
+          for (int kb = 0; kb < x.blocks; ++kb) {
             if (!mbar_wait(full_bar(s), ph, status, 0x44)) {
               *abort_flag = 1;
               ok = false;
-              break;
+              return;
             }
             tc_fence_after();
             const u32 sx = base + s * C::STAGE_BYTES, sy = sx + C::A_BYTES;
-            const int steps = C::GROUPED && x.tail && kb == x.nkb - 1 ? (x.tail + C::UMMA_K - 1) / C::UMMA_K
-                                                                      : C::BK / C::UMMA_K;
+            const auto mma = [&](int k) {
+              mma2_f16_ss(d_tmem, smem_desc_sw128(sx + k * C::UMMA_K * 128, C::CHUNK_BYTES, 1024),
+                          smem_desc_sw128(sy + k * C::UMMA_K * 128, C::CHUNK_BYTES, 1024), idesc,
+                          (kb > 0 || k > 0) ? 1u : 0u);
+            };
+            if (kb < x.blocks - 1 || x.last == 4) {
 #pragma unroll
-            for (int k = 0; k < C::BK / C::UMMA_K; ++k) {
-              if (C::GROUPED && k >= steps) break;
-              const u64 ad = smem_desc_sw128(sx + k * C::UMMA_K * 128, C::CHUNK_BYTES, 1024);
-              const u64 bd = smem_desc_sw128(sy + k * C::UMMA_K * 128, C::CHUNK_BYTES, 1024);
-              mma2_f16_ss(d_tmem, ad, bd, idesc, (kb > 0 || k > 0) ? 1u : 0u);
+              for (int k = 0; k < 4; ++k) mma(k);
+            } else {
+              for (int k = 0; k < x.last; ++k) mma(k);
             }
             tc_commit2(mapa_cluster(empty_bar(s), 0));
             tc_commit2(mapa_cluster(empty_bar(s), 1));
@@ -931,6 +1012,22 @@ __global__ void __launch_bounds__(C::THREADS, 1)
               s = 0;
               ph ^= 1u;
             }
+          }
+          if (x.rest) {
+            const int b = shorts & 1;
+            if (!mbar_wait(short_ready(b), (shorts >> 1) & 1, status, 0x49)) {
+              *abort_flag = 1;
+              ok = false;
+              return;
+            }
+            ++shorts;
+            tc_fence_after();
+            const u32 sx = base + C::SHORT_OFF + b * C::SHORT_BYTES;
+            mma2_f16_ss(d_tmem, smem_desc_sw128(sx, C::SHORT_CHUNK, 1024),
+                        smem_desc_sw128(sx + 2 * C::SHORT_CHUNK, C::SHORT_CHUNK, 1024), idesc,
+                        x.blocks ? 1u : 0u);
+            tc_commit2(mapa_cluster(short_empty(b), 0));
+            tc_commit2(mapa_cluster(short_empty(b), 1));
           }
         };
         if (x.chunks == 2)
@@ -950,54 +1047,49 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     // ------------------------------------------------ rows behind a group's end
     OuterWalk<C> walk(g, tab_off);
     OuterTile x;
-    int s = 0;
-    u32 uses = 0;  // bit s: parity of the next use of stage s's tail barriers
+    int shorts = 0;
     while (!*abort_flag && walk.next(x)) {
-      if (x.nkb == 0) continue;
-      s = (s + x.nkb - 1) % C::STAGES;  // the last k-block's stage
-      if (x.tail) {
-        const u32 par = (uses >> s) & 1u;
-        uses ^= 1u << s;
-        bool ok = true;
-        if (lane == 0) ok = mbar_wait(tail_bar(s), par, status, 0x46);
-        if (!__shfl_sync(0xffffffffu, ok ? 1 : 0, 0)) {
-          *abort_flag = 1;
-          break;
-        }
-        unsigned char *st = smem + s * C::STAGE_BYTES;
-        const int end = (x.tail + C::UMMA_K - 1) / C::UMMA_K * C::UMMA_K;  // rows that an instruction reads
-        const int lines = 2 + x.chunks;                                    // 128-byte columns of both operands
-        for (int i = x.tail * 8 + lane; i < end * 8; i += 32)
-          for (int c = 0; c < lines; ++c)
-            *reinterpret_cast<uint4 *>(st + c * C::CHUNK_BYTES + i * 16) = make_uint4(0, 0, 0, 0);
-        fence_proxy_async_smem();  // the MMA reads through the async proxy
-        __syncwarp();
-        if (lane == 0) {
-          if (rank != 0) {
-            mbar_arrive_cluster(fixed_bar(s), 0);
-          } else {
-            if (!mbar_wait(fixed_bar(s), par, status, 0x47)) *abort_flag = 1;
-            fence_proxy_async_smem();
-            mbar_arrive(full_bar(s));
-          }
-        }
-        __syncwarp();
+      if (!x.rest) continue;
+      const int b = shorts & 1;
+      const u32 par = (shorts >> 1) & 1;
+      ++shorts;
+      bool ok = true;
+      if (lane == 0) ok = mbar_wait(short_full(b), par, status, 0x46);
+      if (!__shfl_sync(0xffffffffu, ok ? 1 : 0, 0)) {
+        *abort_flag = 1;
+        break;
       }
-      s = (s + 1) % C::STAGES;
+      unsigned char *at = smem + C::SHORT_OFF + b * C::SHORT_BYTES;
+      for (int i = x.rest * 8 + lane; i < C::UMMA_K * 8; i += 32)
+        for (int c = 0; c < 2 + x.chunks; ++c)
+          *reinterpret_cast<uint4 *>(at + c * C::SHORT_CHUNK + i * 16) = make_uint4(0, 0, 0, 0);
+      fence_proxy_async_smem();  // the MMA reads through the async proxy
+      __syncwarp();
+      if (lane == 0) {
+        if (rank != 0) {
+          mbar_arrive_cluster(short_peer(b), 0);
+        } else {
+          if (!mbar_wait(short_peer(b), par, status, 0x47)) *abort_flag = 1;
+          fence_proxy_async_smem();
+          mbar_arrive(short_ready(b));
+        }
+      }
+      __syncwarp();
     }
   } else {
     // ------------------------------------------------ epilogue (both CTAs)
     const int q = warp & 3;            // TMEM lane quadrant this warp may access
     const int half = (warp - 2) >> 2;  // takes 32-column slices half, half + 2, ...
-    unsigned char *stg = smem + C::STG_OFF + (warp - 2) * 2048;
+    unsigned char *stg = smem + C::STG_OFF + (warp - 2) * 4096;
+    const u32 stg_at = base + C::STG_OFF + (warp - 2) * 4096;
     OuterWalk<C> walk(g, tab_off);
     OuterTile x;
     int it = 0;
     while (!*abort_flag && walk.next(x)) {
-      unsigned short *out = g.epi.out + static_cast<long long>(x.grp) * g.GM * g.GN;
+      const bool some = x.blocks || x.rest;
       const int row0 = x.m0 + rank * C::BM + q * 32;
       const int acc = it & 1;
-      if (x.nkb) {
+      if (some) {
         bool ok = true;
         if (lane == 0) ok = mbar_wait(tfull_bar(acc), (it >> 1) & 1, status, 0x48);
         if (!__shfl_sync(0xffffffffu, ok ? 1 : 0, 0)) {
@@ -1007,34 +1099,39 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         tc_fence_after();
       }
       const u32 t_row = tmem_base + (static_cast<u32>(q * 32) << 16) + acc * (C::TMEM_COLS / 2);
-      // thread = row: a row's 32 columns leave through this warp's staging
-      // block (rows of 64 bytes, chunks as in rows_kernel's)
 #pragma unroll 1
-      for (int i = half; i < 4 * x.chunks; i += 2) {
-        const int col0 = x.n0 + 32 * i;
+      for (int i = half; i < 2 * x.chunks; i += 2) {
+        const int col0 = x.n0 + 64 * i;
         if (row0 >= g.GM || col0 >= g.GN) break;
-        u32 r[32];
-        if (x.nkb) {
-          tmem_ld_32x32b_x32(t_row + 32 * i, r);
-          tmem_wait_ld();
+        u32 w[32];  // thread = row: 64 columns as bf16
+        if (some) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            u32 r[32];
+            tmem_ld_32x32b_x32(t_row + 64 * i + 32 * h, r);
+            tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              w[16 * h + j] = pack_bf16x2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
+          }
         } else {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) r[j] = 0u;
+          for (int j = 0; j < 32; ++j) w[j] = 0u;
         }
+        if (lane == 0) bulk_wait_read<0>();  // the slice before has left the staging block
+        __syncwarp();
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          u32 w[4];
-#pragma unroll
-          for (int h = 0; h < 4; ++h)
-            w[h] = pack_bf16x2(__uint_as_float(r[8 * j + 2 * h]), __uint_as_float(r[8 * j + 2 * h + 1]));
-          *reinterpret_cast<uint4 *>(stg + lane * 64 + ((j ^ ((lane >> 1) & 3)) * 16)) =
-              make_uint4(w[0], w[1], w[2], w[3]);
+        for (int j = 0; j < 8; ++j)
+          *reinterpret_cast<uint4 *>(stg + lane * 128 + ((j ^ (lane & 7)) * 16)) =
+              make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_3d(&tmap_out, stg_at, col0, row0, x.grp);
+          bulk_commit();
         }
-        __syncwarp();
-        store_block(stg, out, g.GN, row0, g.GM, col0, lane);
-        __syncwarp();
       }
-      if (x.nkb) {
+      if (some) {
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
@@ -1046,6 +1143,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         ++it;
       }
     }
+    if (lane == 0) bulk_wait<0>();
   }
 
   __syncwarp();

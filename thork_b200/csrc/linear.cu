@@ -168,25 +168,31 @@ int weight_gradient(const void *x, const void *dy, int rows, int n, int k, const
   using C = OuterCfg<GROUPED>;
   static std::atomic<uint64_t> done{0};
   int rc, sms;
-  alignas(64) TensorMap tx, ty;
-  if ((rc = thork_encode_tmap_3d(&tx, THORK_DT_BF16, x, k, rows, 1, C::CHUNK, C::BK))) return rc;
-  if ((rc = thork_encode_tmap_3d(&ty, THORK_DT_BF16, dy, n, rows, 1, C::CHUNK, C::BK))) return rc;
+  alignas(64) TensorMap tx, ty, tx16, ty16, tout;
+  const auto map = [&](TensorMap &t, const void *p, int cols, int box_rows) {
+    return thork_encode_tmap_3d(&t, THORK_DT_BF16, p, cols, rows, 1, C::CHUNK, box_rows);
+  };
+  if ((rc = map(tx, x, k, C::BK)) || (rc = map(ty, dy, n, C::BK))) return rc;
+  if ((rc = map(tx16, x, k, C::UMMA_K)) || (rc = map(ty16, dy, n, C::UMMA_K))) return rc;
+  if ((rc = thork_encode_tmap_3d(&tout, THORK_DT_BF16, g.epi.out, n, k, GROUPED ? g.groups : 1, C::CHUNK, 32)))
+    return rc;
   auto kern = outer_kernel<C>;
   if ((rc = allow_smem(reinterpret_cast<const void *>(kern), C::SMEM_BYTES, done))) return rc;
   if ((rc = thork_sm_count(&sms))) return rc;
   // one pair per half of a tile at most
   const long long most = 2ll * ((k + 255) / 256) * ((n + 255) / 256) * (GROUPED ? g.groups : 1);
   const int pairs = static_cast<int>(most < sms / 2 ? most : sms / 2);
-  return launch(kern, 2 * pairs, C::THREADS, C::SMEM_BYTES, 2, s, what, tx, ty, g);
+  return launch(kern, 2 * pairs, C::THREADS, C::SMEM_BYTES, 2, s, what, tx, ty, tx16, ty16, tout, g);
 }
 
 int slope(SlopeArgs a, cudaStream_t s, const char *what) {
   int rc, sms;
   if ((rc = thork_sm_count(&sms))) return rc;
   const long long stripes = (a.cols + 127) / 128;
-  // two waves of four blocks per SM, at most one per 32 rows; the column
-  // sums' blocks are a cluster, of at most eight
-  long long split = (8ll * sms + stripes - 1) / stripes;
+  // one wave of four blocks per SM, at most one per 32 rows; the column sums'
+  // blocks are a cluster, of at most eight
+  long long split = 4ll * sms / stripes;
+  if (split < 1) split = 1;
   const long long most = (a.rows + 31) / 32;
   if (split > most) split = most;
   if (a.dbias && split > 8) split = 8;
