@@ -81,6 +81,27 @@ __device__ __forceinline__ void tma_store_3d(const TensorMap *m, u32 src, int x,
       : "memory");
 }
 
+// Arrive on `bar`, at the same shared-memory offset in both CTAs of a pair,
+// when the tcgen05 operations issued so far by this thread are complete.
+__device__ __forceinline__ void tc_commit_pair(u32 bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          bar),
+      "h"(static_cast<unsigned short>(3))
+      : "memory");
+}
+
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  u32 p;
+  asm volatile(
+      "{\n\t.reg .pred P;\n\t"
+      "elect.sync _|P, 0xffffffff;\n\t"
+      "selp.b32 %0, 1, 0, P;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+
 __device__ __forceinline__ u32 cluster_nctarank() {
   u32 r;
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
@@ -531,9 +552,10 @@ __global__ void __launch_bounds__(C::THREADS, 1)
 
   if (warp == 0) {
     // ------------------------------------------------ TMA producer (both CTAs)
-    if (lane == 0) {
+    if (elect_one()) {
       RowWalk<C> walk(g, tab_off, tab_tile);
       RowTile x;
+      const u32 leader_full = mapa_cluster(full_bar(0), 0);
       int s = 0;
       u32 ph = 0;
       while (!*abort_flag && walk.next(x)) {
@@ -545,7 +567,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
             break;
           }
           const u32 sw = base + s * C::STAGE_BYTES, sx = sw + C::W_BYTES;
-          const u32 fb = mapa_cluster(full_bar(s), 0);
+          const u32 fb = leader_full + 8u * s;
           if (rank == 0) mbar_arrive_expect_tx(full_bar(s), bytes);
           if (C::W_MN) {
 #pragma unroll
@@ -580,7 +602,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
   } else if (warp == 1) {
     // ------------------------------------------------ MMA issuer (leader CTA)
     // all of it in lane 0: a warp-wide step per k-block idles the tensor pipe
-    if (rank == 0 && lane == 0) {
+    if (rank == 0 && elect_one()) {
       RowWalk<C> walk(g, tab_off, tab_tile);
       RowTile x;
       int s = 0, it = 0;
@@ -617,8 +639,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
               else
                 mma2_f8f6f4_ss(d_tmem, ad, bd, idesc, accum);
             }
-            tc_commit2(mapa_cluster(empty_bar(s), 0));
-            tc_commit2(mapa_cluster(empty_bar(s), 1));
+            tc_commit_pair(empty_bar(s));
             if (++s == C::STAGES) {
               s = 0;
               ph ^= 1u;
@@ -634,8 +655,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         else
           run(Const<1>());
         if (!ok || *abort_flag) break;
-        tc_commit2(mapa_cluster(tfull_bar(acc), 0));
-        tc_commit2(mapa_cluster(tfull_bar(acc), 1));
+        tc_commit_pair(tfull_bar(acc));
         ++it;
       }
       tc_commit2(mapa_cluster(drain_bar, 0));
@@ -914,9 +934,10 @@ __global__ void __launch_bounds__(C::THREADS, 1)
 
   if (warp == 0) {
     // ------------------------------------------------ TMA producer (both CTAs)
-    if (lane == 0) {
+    if (elect_one()) {
       OuterWalk<C> walk(g, tab_off);
       OuterTile x;
+      const u32 leader_full = mapa_cluster(full_bar(0), 0);
       int s = 0, shorts = 0;
       u32 ph = 0;
       while (!*abort_flag && walk.next(x)) {
@@ -944,7 +965,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
           }
           const u32 sx = base + s * C::STAGE_BYTES, sy = sx + C::A_BYTES;
           if (rank == 0) mbar_arrive_expect_tx(full_bar(s), bytes);
-          const u32 fb = mapa_cluster(full_bar(s), 0);
+          const u32 fb = leader_full + 8u * s;
           const int row = x.r0 + kb * C::BK;
           tma_load_3d_pair(sx, &tmap_x, fb, m, row, 0);
           tma_load_3d_pair(sx + C::CHUNK_BYTES, &tmap_x, fb, m + C::CHUNK, row, 0);
@@ -970,7 +991,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
   } else if (warp == 1) {
     // ------------------------------------------------ MMA issuer (leader CTA)
     // all of it in lane 0: a warp-wide step per k-block idles the tensor pipe
-    if (rank == 0 && lane == 0) {
+    if (rank == 0 && elect_one()) {
       OuterWalk<C> walk(g, tab_off);
       OuterTile x;
       int s = 0, it = 0, shorts = 0;
@@ -1006,8 +1027,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
             } else {
               for (int k = 0; k < x.last; ++k) mma(k);
             }
-            tc_commit2(mapa_cluster(empty_bar(s), 0));
-            tc_commit2(mapa_cluster(empty_bar(s), 1));
+            tc_commit_pair(empty_bar(s));
             if (++s == C::STAGES) {
               s = 0;
               ph ^= 1u;
@@ -1026,8 +1046,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
             mma2_f16_ss(d_tmem, smem_desc_sw128(sx, C::SHORT_CHUNK, 1024),
                         smem_desc_sw128(sx + 2 * C::SHORT_CHUNK, C::SHORT_CHUNK, 1024), idesc,
                         x.blocks ? 1u : 0u);
-            tc_commit2(mapa_cluster(short_empty(b), 0));
-            tc_commit2(mapa_cluster(short_empty(b), 1));
+            tc_commit_pair(short_empty(b));
           }
         };
         if (x.chunks == 2)
@@ -1035,8 +1054,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         else
           run(Const<1>());
         if (!ok || *abort_flag) break;
-        tc_commit2(mapa_cluster(tfull_bar(acc), 0));
-        tc_commit2(mapa_cluster(tfull_bar(acc), 1));
+        tc_commit_pair(tfull_bar(acc));
         ++it;
       }
       tc_commit2(mapa_cluster(drain_bar, 0));
@@ -1276,7 +1294,7 @@ __global__ void __launch_bounds__(C::THREADS)
 
   if (live) {
     if (warp == 0) {
-      if (lane == 0) {
+      if (elect_one()) {
         // weights that no earlier kernel writes are fetched for the opening
         // stages while the previous kernel of the stream still runs
         int pre = 0;
@@ -1303,7 +1321,7 @@ __global__ void __launch_bounds__(C::THREADS)
         }
       }
     } else if (warp == 1) {
-      if (lane == 0) {
+      if (elect_one()) {
         int s = 0;
         u32 ph = 0;
         for (int kb = kb0; kb < kb1; ++kb) {
