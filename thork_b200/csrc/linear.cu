@@ -82,10 +82,6 @@ struct Product {
   int groups;      // 0: dense
 };
 
-// k-blocks per CTA below which splitting the contraction further costs more
-// (one more partial tile to sum) than its shorter loop saves
-constexpr int kMinSplitBlocks = 4;
-
 template <int KIND, bool W_MN>
 int map_w(TensorMap &t, const Product &p, int box_n) {
   const int elem = KIND == KIND_BF16 ? 2 : 1;
@@ -104,29 +100,20 @@ int map_x(TensorMap &t, const Product &p, int box_rows) {
 }
 
 template <int KIND, int BN, int STAGES, bool W_MN, bool GROUPED>
-int swap_product(const Product &p, const GemmArgs &g, cudaStream_t s, const char *what) {
+int swap_product(const Product &p, const GemmArgs &g, int split, cudaStream_t s, const char *what) {
   using C = SwapCfg<KIND, BN, STAGES, W_MN, GROUPED>;
-  int rc, sms;
+  int rc;
   alignas(64) TensorMap tw, tx;
   if ((rc = map_w<KIND, W_MN>(tw, p, C::BM))) return rc;
   if ((rc = map_x<KIND>(tx, p, BN))) return rc;
-  if ((rc = thork_sm_count(&sms))) return rc;
   const long long ntn = (p.n + C::BM - 1) / C::BM;
-  long long rt = (p.rows + BN - 1) / BN, likely = rt;
+  long long rt = (p.rows + BN - 1) / BN;
   if (GROUPED) {
     // at most one partial tile per group that has rows
     const long long most = (static_cast<long long>(p.rows) + static_cast<long long>(p.groups) * (BN - 1)) / BN;
     rt = most < p.rows ? most : p.rows;
-    const long long held = p.groups < p.rows ? p.groups : p.rows;
-    likely = likely > held ? likely : held;
   }
-  // two CTAs fit on an SM: split the contraction until they are all in use
-  const int nkb = (p.k + C::BK - 1) / C::BK;
-  long long split = 2ll * sms / (likely * ntn);
-  if (split > nkb / kMinSplitBlocks) split = nkb / kMinSplitBlocks;
-  if (split > 8) split = 8;
-  if (split < 1) split = 1;
-  return run_swap<C>(tw, tx, g, rt * ntn, static_cast<int>(split), s, what);
+  return run_swap<C>(tw, tx, g, rt * ntn, split, s, what);
 }
 
 template <int KIND, bool W_MN, bool GROUPED>
@@ -149,16 +136,94 @@ int rows_product(const Product &p, const GemmArgs &g, cudaStream_t s, const char
   return launch(kern, 2 * pairs, C::THREADS, C::SMEM_BYTES, 2, s, what, tw, tx, txu, g);
 }
 
-template <int KIND, bool W_MN, bool GROUPED>
-int product(const Product &p, const GemmArgs &g, cudaStream_t s, const char *what) {
-  // rows that a tile can expect: of the whole product, or of one group
-  const long long rows = GROUPED ? (static_cast<long long>(p.rows) + p.groups - 1) / p.groups : p.rows;
-  constexpr int G = GROUPED ? 1 : 0;  // the group table takes one stage's room
-  if (rows <= 16) return swap_product<KIND, 16, 6 - G, W_MN, GROUPED>(p, g, s, what);
-  if (rows <= 32) return swap_product<KIND, 32, 5, W_MN, GROUPED>(p, g, s, what);
-  if (rows <= 64) return swap_product<KIND, 64, 4, W_MN, GROUPED>(p, g, s, what);
-  if (rows <= 128) return swap_product<KIND, 128, 3, W_MN, GROUPED>(p, g, s, what);
-  return rows_product<KIND, W_MN, GROUPED>(p, g, s, what);
+// ---------------------------------------------------------------- choice of kernel
+// Microseconds of one dense product by each kernel, estimated.  The forms and
+// constants were fitted to 4050 products timed on B200 with every choice (M 1
+// to 1600, N and K 128 to 14336, bf16); picking by them is 1 % (mean) from the
+// best choice of each beyond the timing's noise.  Some of the sides, measured
+// (us; swap_kernel with BN rows a tile and the contraction split in S):
+//     M    N     K    rows  swap (BN/S)      M    N     K    rows  swap (BN/S)
+//     1  4096  4096   18.7   10.8 (16/4)    256  4096  4096   19.4   17.0 (128/4)
+//    64  1544  1032    8.8    6.8 (32/4)    256 14336  4096   29.4   40.0 (128/1)
+//   128  4096  4096   19.2   13.4 (64/4)    512   512  8192   32.7   15.3 (128/8)
+//   128 14336  4096   25.1   30.1 (128/2)   777  1544  1032   10.6   14.5 (128/2)
+constexpr int ceil_div(long long a, int b) { return static_cast<int>((a + b - 1) / b); }
+
+double rows_us(int nkb, int m, int n, double mbytes, int pairs) {
+  int units = ceil_div(m, 64);
+  if (units > 4) units = 4;
+  const long long tiles = static_cast<long long>(ceil_div(m, 256)) * ceil_div(n, 256);
+  double waves = 1.0;
+  if (tiles < pairs) {
+    const int pieces = static_cast<int>(pairs / tiles < 4 ? pairs / tiles : 4);
+    units = ceil_div(units, pieces);
+  } else {
+    const int rest = static_cast<int>(tiles % pairs);
+    const int pieces = rest ? (pairs / rest < 4 ? pairs / rest : 4) : 1;
+    waves = static_cast<double>(tiles / pairs) + (rest ? (pieces > 1 ? 0.7 : 1.0) : 0.0);
+  }
+  const double block = 0.07 * units > 0.3 ? 0.07 * units : 0.3;
+  const double math = waves * (nkb * block + 0.2), memory = mbytes / 7.0;
+  return 5.2 + (math > memory ? math : memory);
+}
+
+double swap_us(int nkb, int m, int n, double mbytes, int sms, int bn, int split) {
+  const double ctas = static_cast<double>(ceil_div(m, bn)) * ceil_div(n, 128) * split;
+  double waves = static_cast<double>(static_cast<long long>(ctas / (2 * sms) + 0.95));
+  if (waves < 1.0) waves = 1.0;
+  // two CTAs of an SM share its feed: a stage is 16 KiB of weights and 128 bytes a row
+  const double shared = ctas > 2 * sms ? 2.0 : ctas > sms ? ctas / sms : 1.0;
+  const double feed = 0.6 * (16 + bn / 8) / 32 * shared;
+  const double math = waves * (ceil_div(nkb, split) * (feed > 0.26 ? feed : 0.26) + 0.15), memory = mbytes / 6.3;
+  const double height = (m < bn ? m : bn) / 16.0;
+  return 5.1 + height * (0.32 * (split > 1 ? 1.3 : 1.0) + 0.02 * split) + (math > memory ? math : memory);
+}
+
+template <int KIND, bool W_MN>
+int dense_product(const Product &p, const GemmArgs &g, cudaStream_t s, const char *what) {
+  int rc, sms;
+  if ((rc = thork_sm_count(&sms))) return rc;
+  const int elem = KIND == KIND_BF16 ? 2 : 1, nkb = ceil_div(p.k, 128 / elem);
+  const double mbytes = (elem * (static_cast<double>(p.n) * p.k + static_cast<double>(p.rows) * p.k) +
+                         2.0 * p.rows * p.n) * 1e-6;
+  double best = rows_us(nkb, p.rows, p.n, mbytes, sms / 2);
+  int bn = 0, split = 0;
+  for (int b = 16; b <= 128; b *= 2)
+    for (int c = 1; c <= 8 && 2 * c <= nkb + 1; c *= 2) {
+      const double us = swap_us(nkb, p.rows, p.n, mbytes, sms, b, c);
+      if (us < best) {
+        best = us;
+        bn = b;
+        split = c;
+      }
+    }
+  switch (bn) {
+    case 16: return swap_product<KIND, 16, 6, W_MN, false>(p, g, split, s, what);
+    case 32: return swap_product<KIND, 32, 5, W_MN, false>(p, g, split, s, what);
+    case 64: return swap_product<KIND, 64, 4, W_MN, false>(p, g, split, s, what);
+    case 128: return swap_product<KIND, 128, 3, W_MN, false>(p, g, split, s, what);
+    default: return rows_product<KIND, W_MN, false>(p, g, s, what);
+  }
+}
+
+// The groups' sizes are on the device, so the rule goes by their mean.  Few
+// rows a group: swap_kernel, whose tiles waste no instruction on rows that are
+// not there; more: rows_kernel (us, mean rows 2 / 8 / 31 / 63: E=8 of 14336 x
+// 4096 126 against 131 with rows_kernel; E=64 of 2048 x 2048 86 / 85; E=37 of
+// 760 x 1304 28.6 / 22.3; e4m3 E=64 of 2048 x 1024 48 / 35).
+template <int KIND, bool W_MN>
+int grouped_product(const Product &p, const GemmArgs &g, cudaStream_t s, const char *what) {
+  int rc, sms;
+  if ((rc = thork_sm_count(&sms))) return rc;
+  const int mean = ceil_div(p.rows, p.groups);
+  if (mean > 24) return rows_product<KIND, W_MN, true>(p, g, s, what);
+  // two CTAs fit on an SM: split the contraction until they are all in use
+  const long long held = p.groups < p.rows ? p.groups : p.rows;
+  const int nkb = ceil_div(p.k, KIND == KIND_BF16 ? 64 : 128);
+  int split = 1;
+  while (split < 8 && 2 * split * held * ceil_div(p.n, 128) <= 2 * sms && 4 * split <= nkb) split *= 2;
+  if (mean <= 4) return swap_product<KIND, 16, 5, W_MN, true>(p, g, split, s, what);
+  return swap_product<KIND, 32, 5, W_MN, true>(p, g, split, s, what);
 }
 
 // dW[k, n] = sum over rows X[m, k] dY[m, n], of each group's rows when grouped.
@@ -270,7 +335,7 @@ int linear(const void *a, const void *b, void *c, const void *bias, const void *
   g.GN = N;
   g.GK = K;
   g.w_static = flags & THORK_LINEAR_W_STATIC;
-  return product<KIND, true, false>({a, b, M, N, K, 0}, g, static_cast<cudaStream_t>(stream), what);
+  return dense_product<KIND, true>({a, b, M, N, K, 0}, g, static_cast<cudaStream_t>(stream), what);
 }
 
 template <int KIND>
@@ -297,7 +362,7 @@ int grouped(const void *a, const void *b, void *c, const int *offsets, void *pre
   g.GK = K;
   g.offsets = offsets;
   g.groups = E;
-  return product<KIND, true, true>({a, b, T, N, K, E}, g, static_cast<cudaStream_t>(stream), what);
+  return grouped_product<KIND, true>({a, b, T, N, K, E}, g, static_cast<cudaStream_t>(stream), what);
 }
 
 // Gradients of a (grouped) linear layer from dout and, with an activation,
@@ -339,7 +404,7 @@ int backward(void *da, void *db, float *dbias, const void *dout, const void *a, 
     d.GN = K;
     d.GK = N;
     const Product p = {dz, b, rows, K, N, groups};
-    rc = groups ? product<KIND_BF16, false, true>(p, d, s, what) : product<KIND_BF16, false, false>(p, d, s, what);
+    rc = groups ? grouped_product<KIND_BF16, false>(p, d, s, what) : dense_product<KIND_BF16, false>(p, d, s, what);
     if (rc) return rc;
   }
   if (db) {
