@@ -362,12 +362,25 @@ struct RowWalk {
     whole = total - rest;
     pieces = rest ? min(C::MAX_UNITS, step / rest) : 1;
     items = whole + rest * pieces;
+    more = find(ahead);
   }
   static __device__ __forceinline__ int row_tiles(int rows) {
     return (rows + C::UNIT * C::MAX_UNITS - 1) / (C::UNIT * C::MAX_UNITS);
   }
 
+  // The next tile; the one after it is worked out here as well, while the
+  // caller's first wait would still be pending, so that the arithmetic stays
+  // off the path from one tile's end to the next one's start.
+  RowTile ahead;
+  bool more;
   __device__ __forceinline__ bool next(RowTile &x) {
+    if (!more) return false;
+    x = ahead;
+    more = find(ahead);
+    return true;
+  }
+
+  __device__ __forceinline__ bool find(RowTile &x) {
     for (; i < items; i += step) {
       int t = i, piece = 0, parts = 1;
       if (i >= whole && pieces > 1) {
@@ -832,9 +845,19 @@ struct OuterWalk {
     whole = total - rest;
     halves = 2 * rest <= step;
     items = whole + rest * (halves ? 2 : 1);
+    more = find(ahead);
   }
 
+  OuterTile ahead;  // worked out one tile early, as in RowWalk
+  bool more;
   __device__ __forceinline__ bool next(OuterTile &x) {
+    if (!more) return false;
+    x = ahead;
+    more = find(ahead);
+    return true;
+  }
+
+  __device__ __forceinline__ bool find(OuterTile &x) {
     for (; i < items; i += step) {
       int t = i, part = 0;
       x.chunks = 2;
