@@ -91,6 +91,16 @@ __device__ __forceinline__ void tc_commit_pair(u32 bar) {
       : "memory");
 }
 
+// An epilogue warp hands its accumulator columns back to the MMA thread of the
+// pair's leader (`bar_cluster` in its shared memory).  What is ordered are the
+// tensor-memory loads, which have completed and which
+// tcgen05.fence::before_thread_sync orders before this arrival, so it need not
+// release memory: as a release of cluster scope it waited for every store in
+// flight (outer_kernel: 2000 of 4500 cycles between short tiles).
+__device__ __forceinline__ void arrive_tmem_free(u32 bar_cluster) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
+}
+
 // One lane of a converged warp.
 __device__ __forceinline__ bool elect_one() {
   u32 p;
@@ -682,6 +692,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     const Epilogue &p = g.epi;
     unsigned char *stg = smem + C::STG_OFF + (warp - 2) * 2048;
     const u32 stg_at = base + C::STG_OFF + (warp - 2) * 2048;
+    const u32 leader_tempty = mapa_cluster(tempty_bar(0), 0);
     RowWalk<C> walk(g, tab_off, tab_tile);
     RowTile x;
     int it = 0;
@@ -747,10 +758,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
-        if (rank == 0)
-          mbar_arrive(tempty_bar(acc));
-        else
-          mbar_arrive_cluster(tempty_bar(acc), 0);
+        arrive_tmem_free(leader_tempty + 8u * acc);
       }
       ++it;
     }
@@ -1123,6 +1131,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     const int half = (warp - 2) >> 2;  // takes 32-column slices half, half + 2, ...
     unsigned char *stg = smem + C::STG_OFF + (warp - 2) * 4096;
     const u32 stg_at = base + C::STG_OFF + (warp - 2) * 4096;
+    const u32 leader_tempty = mapa_cluster(tempty_bar(0), 0);
     OuterWalk<C> walk(g, tab_off);
     OuterTile x;
     int it = 0;
@@ -1176,10 +1185,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
-          if (rank == 0)
-            mbar_arrive(tempty_bar(acc));
-          else
-            mbar_arrive_cluster(tempty_bar(acc), 0);
+          arrive_tmem_free(leader_tempty + 8u * acc);
         }
         ++it;
       }
