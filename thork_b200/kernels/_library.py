@@ -93,26 +93,24 @@ class Operand:
     element type, shape and whether the call writes it (``partly``: not all of
     it, so that a host array's contents go in as well)."""
 
-    __slots__ = ("name", "dtype", "shape", "count", "written", "partly", "_ok")
+    __slots__ = ("name", "dtype", "shape", "count", "written", "partly", "seen")
 
     def __init__(self, name: str, dtype: dt.Dtype, shape: Tuple[int, ...], written: bool = False,
                  partly: bool = False):
         self.name, self.dtype, self.shape = name, dtype, tuple(shape)
         self.count = math.prod(shape)
         self.written, self.partly = written, partly
-        self._ok = set()  # storage dtypes that have been accepted before
+        self.seen = None  # a storage dtype that has passed the check before
 
     def check(self, a, dev: int) -> None:
         host = isinstance(a, np.ndarray)
         if not host and not isinstance(a, rt.DeviceArray):
             raise TypeError(f"Argument for '{self.name}' must be a numpy array or a DeviceArray, got "
                             f"{type(a).__name__}")
-        if a.dtype not in self._ok:
-            if not dt.storage_compatible(a.dtype, self.dtype):
-                raise TypeError(f"Argument for '{self.name}' has dtype {a.dtype}, expected "
-                                f"{self.dtype.name}")
-            self._ok.add(a.dtype)
-        if math.prod(a.shape) != self.count:
+        if not dt.storage_compatible(a.dtype, self.dtype):
+            raise TypeError(f"Argument for '{self.name}' has dtype {a.dtype}, expected {self.dtype.name}")
+        self.seen = a.dtype
+        if a.size != self.count:
             raise ValueError(f"Argument for '{self.name}' has shape {tuple(a.shape)}, expected "
                              f"{self.shape}")
         if host:
@@ -130,16 +128,26 @@ def run_operands(operands: Sequence[Operand], args: Sequence, launch: Callable, 
     copies host arrays in and written ones back."""
     dev = rt.get_device()
     s = stream if stream is not None else rt._dispatch_stream()
-    ptrs, owned, back = [], [], []
+    DeviceArray = rt.DeviceArray
+    ptrs, owned, back = [], None, None
     try:
         for o, a in zip(operands, args):
             if a is None:
                 ptrs.append(None)
                 continue
-            o.check(a, dev)
-            if isinstance(a, rt.DeviceArray):
+            # the checks of an array that passes them, in line: a call's host
+            # time shows when its kernel takes a few microseconds
+            if type(a) is DeviceArray:
+                if a.dtype is not o.seen or a.size != o.count or a.buffer._dev != dev:
+                    o.check(a, dev)
                 ptrs.append(a.buffer.ptr)
                 continue
+            o.check(a, dev)
+            if isinstance(a, DeviceArray):
+                ptrs.append(a.buffer.ptr)
+                continue
+            if owned is None:
+                owned, back = [], []
             buf = rt.DeviceBuffer(a.nbytes)
             owned.append(buf)
             ptrs.append(buf.ptr)
@@ -147,14 +155,19 @@ def run_operands(operands: Sequence[Operand], args: Sequence, launch: Callable, 
                 rt.copy_htod(buf.ptr, a, s, sync=False)
             if o.written:
                 back.append((a, buf.ptr))
-        rt.check(launch(ptrs, s.handle), what)
-        for a, ptr in back:
-            rt.copy_dtoh(a, ptr, s, sync=False)
-        if sync or owned:
+        rc = launch(ptrs, s.handle)
+        if rc:
+            rt.check(rc, what)
+        if owned is not None:
+            for a, ptr in back:
+                rt.copy_dtoh(a, ptr, s, sync=False)
+            s.synchronize()
+        elif sync:
             s.synchronize()
     finally:
-        for b in owned:
-            b.free()
+        if owned is not None:
+            for b in owned:
+                b.free()
 
 
 class LibraryKernel:

@@ -18,6 +18,7 @@ There is no CPU fallback: if the library or a GPU is missing, calls raise.
 
 import ctypes
 import hashlib
+import math
 import os
 import re
 import struct
@@ -398,7 +399,8 @@ class DeviceArray:
     def __init__(self, shape, dtype, buffer: Optional[DeviceBuffer] = None):
         self.shape = tuple(int(s) for s in shape)
         self.dtype = np.dtype(dtype)
-        self.nbytes = int(np.prod(self.shape, dtype=np.int64)) * self.dtype.itemsize
+        self.size = math.prod(self.shape)
+        self.nbytes = self.size * self.dtype.itemsize
         self.buffer = buffer if buffer is not None else DeviceBuffer(self.nbytes)
 
     @property
