@@ -52,6 +52,12 @@ struct GemmArgs {
   const int *offsets;  // [groups + 1] row offsets, or null
   int groups, rows;    // groups, rows of the buffer that the offsets divide
   int w_static;        // swap_kernel: no earlier launch writes the weights
+  // Two products of one call that do not read each other's output overlap: the
+  // first (trigger_late) lets the second start only once everything before the
+  // first has completed, so that the second (wait_last) needs no wait of its
+  // own before it reads; it waits for the first before it ends, so whatever
+  // follows it follows both.
+  int trigger_late, wait_last;
 };
 
 // ---------------------------------------------------------------- small PTX
@@ -568,10 +574,11 @@ __global__ void __launch_bounds__(C::THREADS, 1)
   __syncthreads();
   cluster_sync();  // both CTAs' barriers are initialised before any remote use
   tc_fence_after();
-  pdl_launch_dependents();
+  if (!g.trigger_late) pdl_launch_dependents();
   const u32 tmem_base = *tmem_slot;
   const int nkb = (g.GK + C::BK - 1) / C::BK;
   pdl_wait();  // the previous kernel of the stream is complete from here on
+  if (g.trigger_late && threadIdx.x == 0) pdl_launch_dependents();
 
   if (warp == 0) {
     // ------------------------------------------------ TMA producer (both CTAs)
@@ -952,7 +959,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     tmem_relinquish<2>();
   }
   if (C::GROUPED && warp == 2) {
-    pdl_wait();  // the offsets may come from the previous kernel of the stream
+    if (!g.wait_last) pdl_wait();  // the offsets may come from the previous kernel of the stream
     scan_groups(g.offsets, g.groups, g.rows, 256, tab_off, nullptr, blockIdx.x == 0 ? status : nullptr);
   }
   tc_fence_before();
@@ -961,7 +968,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
   tc_fence_after();
   pdl_launch_dependents();
   const u32 tmem_base = *tmem_slot;
-  pdl_wait();  // the previous kernel of the stream is complete from here on
+  if (!g.wait_last) pdl_wait();  // the previous kernel of the stream is complete from here on
 
   if (warp == 0) {
     // ------------------------------------------------ TMA producer (both CTAs)
@@ -1196,6 +1203,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
   __syncwarp();
   tc_fence_before();
   __syncthreads();
+  if (g.wait_last) pdl_wait();
   cluster_sync();  // the leader's MMAs into both TMEMs are complete
   tc_fence_after();
   if (warp == 1) tmem_dealloc<2>(tmem_base, C::TMEM_COLS);
@@ -1283,7 +1291,7 @@ __global__ void __launch_bounds__(C::THREADS)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  pdl_launch_dependents();
+  if (!g.trigger_late) pdl_launch_dependents();
   const u32 tmem_base = *tmem_slot;
 
   int m0 = rt * C::BN, row_end = g.GM, grp = 0;
@@ -1334,6 +1342,7 @@ __global__ void __launch_bounds__(C::THREADS)
           }
         }
         pdl_wait();
+        if (g.trigger_late) pdl_launch_dependents();
         int s = 0;
         u32 ph = 0;
         for (int kb = kb0; kb < kb1; ++kb) {

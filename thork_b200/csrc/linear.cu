@@ -238,7 +238,12 @@ int weight_gradient(const void *x, const void *dy, int rows, int n, int k, const
     return thork_encode_tmap_3d(&t, THORK_DT_BF16, p, cols, rows, 1, C::CHUNK, box_rows);
   };
   if ((rc = map(tx, x, k, C::BK)) || (rc = map(ty, dy, n, C::BK))) return rc;
-  if ((rc = map(tx16, x, k, C::UMMA_K)) || (rc = map(ty16, dy, n, C::UMMA_K))) return rc;
+  if (GROUPED) {
+    if ((rc = map(tx16, x, k, C::UMMA_K)) || (rc = map(ty16, dy, n, C::UMMA_K))) return rc;
+  } else {
+    tx16 = tx;  // no short blocks
+    ty16 = ty;
+  }
   if ((rc = thork_encode_tmap_3d(&tout, THORK_DT_BF16, g.epi.out, n, k, GROUPED ? g.groups : 1, C::CHUNK, 32)))
     return rc;
   auto kern = outer_kernel<C>;
@@ -403,6 +408,7 @@ int backward(void *da, void *db, float *dbias, const void *dout, const void *a, 
     d.GM = rows;
     d.GN = K;
     d.GK = N;
+    d.trigger_late = db != nullptr;
     const Product p = {dz, b, rows, K, N, groups};
     rc = groups ? grouped_product<KIND_BF16, false>(p, d, s, what) : dense_product<KIND_BF16, false>(p, d, s, what);
     if (rc) return rc;
@@ -414,6 +420,7 @@ int backward(void *da, void *db, float *dbias, const void *dout, const void *a, 
     w.GM = K;
     w.GN = N;
     w.GK = rows;
+    w.wait_last = da != nullptr;
     rc = groups ? weight_gradient<true>(a, dz, rows, N, K, w, s, what)
                 : weight_gradient<false>(a, dz, rows, N, K, w, s, what);
     if (rc) return rc;
