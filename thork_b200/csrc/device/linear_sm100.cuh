@@ -144,35 +144,113 @@ __device__ __forceinline__ float bf16_hi(u32 w) { return __uint_as_float(w & 0xF
 
 // ---------------------------------------------------------------- activations
 // silu is z * sigmoid(z) and gelu_tanh z * sigmoid(2u): one exponential and one
-// division each, off by a few 2^-22 of the value.  The normal distribution
+// reciprocal each, off by a few 2^-22 of the value.  The normal distribution
 // function of gelu takes Abramowitz and Stegun's rational approximation
 // 7.1.26 of erf (absolute error 1.5e-7), because its exponential is the
-// density's, which the slope needs as well: with erff and expf the slope
-// kernel was bound by its instructions (126 us for 4096 x 14336 against 54 us
-// of traffic).  All of it is far below the bf16 rounding of what is stored.
-// A NaN stays a NaN (relu included).
-__device__ __forceinline__ float gelu_tanh_2u(float z) {
-  return 1.5957691216057308f * z * (1.0f + 0.044715f * z * z);
+// density's, which the slope needs as well.  All of it is far below the bf16
+// rounding of what is stored.  A NaN stays a NaN (relu included).
+//
+// Two values at a time, in the packed fp32 instructions: slope_kernel has
+// about as many instructions to issue as bytes to move (4096 x 14336, gelu:
+// 126 us with erff and expf, 73 with the approximation, 66 packed; its traffic
+// takes 54).
+struct F2 {
+  u64 v;
+};
+__device__ __forceinline__ F2 f2(float lo, float hi) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ F2 f2(float x) { return f2(x, x); }
+__device__ __forceinline__ void split(F2 a, float &lo, float &hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(a.v));
+}
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 operator+(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ F2 exp2_2(F2 a) {
+  float x, y;
+  split(a, x, y);
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x));
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(y));
+  return f2(x, y);
+}
+__device__ __forceinline__ F2 reciprocal2(F2 a) {  // 0 for infinity
+  float x, y;
+  split(a, x, y);
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(x));
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(y));
+  return f2(x, y);
 }
 
-// 1 / x to within 2^-23 or so; 0 for infinity.
-__device__ __forceinline__ float reciprocal(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
+constexpr float kLog2e = 1.4426950408889634f;
 
-__device__ __forceinline__ float sigmoid(float z) { return reciprocal(1.0f + __expf(-z)); }
+// 1 / (1 + 2^-a)
+__device__ __forceinline__ F2 sigmoid_exp2(F2 minus_a) { return reciprocal2(f2(1.0f) + exp2_2(minus_a)); }
 
 // Phi(z), and bell = exp(-z^2 / 2).
-__device__ __forceinline__ float normal_cdf(float z, float &bell) {
-  bell = __expf(-0.5f * z * z);
-  const float t = reciprocal(fmaf(0.3275911f * 0.7071067811865476f, fabsf(z), 1.0f));
+__device__ __forceinline__ F2 normal_cdf(F2 z, F2 &bell) {
+  bell = exp2_2(z * z * f2(-0.5f * kLog2e));
+  float x, y, tx, ty;
+  split(z, x, y);
+  const F2 t = reciprocal2(fma2(f2(0.3275911f * 0.7071067811865476f), f2(fabsf(x), fabsf(y)), f2(1.0f)));
   // half of the approximation's polynomial
-  const float poly =
-      t * (0.127414796f + t * (-0.142248368f + t * (0.7107068705f + t * (-0.7265760135f + t * 0.5307027145f))));
-  const float tail = poly * bell;  // Phi(-|z|)
-  return z < 0.0f ? tail : 1.0f - tail;
+  F2 poly = fma2(t, f2(0.5307027145f), f2(-0.7265760135f));
+  poly = fma2(t, poly, f2(0.7107068705f));
+  poly = fma2(t, poly, f2(-0.142248368f));
+  poly = fma2(t, poly, f2(0.127414796f));
+  split(t * poly * bell, tx, ty);  // Phi(-|z|)
+  return f2(x < 0.0f ? tx : 1.0f - tx, y < 0.0f ? ty : 1.0f - ty);
+}
+
+// -2u log2(e) = z (c0 + c1 z^2) for gelu_tanh's 2u = 2 sqrt(2/pi) (z + 0.044715 z^3)
+constexpr float kTanh0 = 1.5957691216057308f, kTanh1 = kTanh0 * 0.044715f;
+
+__device__ __forceinline__ F2 act_value(F2 z, int act) {
+  F2 bell;
+  switch (act) {
+    case ACT_GELU: return z * normal_cdf(z, bell);
+    case ACT_GELU_TANH:
+      return z * sigmoid_exp2(z * fma2(z * z, f2(-kTanh1 * kLog2e), f2(-kTanh0 * kLog2e)));
+    default: return z * sigmoid_exp2(z * f2(-kLog2e));  // silu
+  }
+}
+
+// Derivative of the activation at z.
+__device__ __forceinline__ F2 act_slope(F2 z, int act) {
+  if (act == ACT_GELU) {
+    F2 bell;
+    const F2 cdf = normal_cdf(z, bell);
+    return fma2(z * f2(0.3989422804014327f), bell, cdf);
+  }
+  if (act == ACT_GELU_TANH) {
+    const F2 zz = z * z;
+    const F2 p = sigmoid_exp2(z * fma2(zz, f2(-kTanh1 * kLog2e), f2(-kTanh0 * kLog2e)));
+    const F2 q = fma2(p, p * f2(-1.0f), p);  // p (1 - p)
+    return fma2(z * q, fma2(zz, f2(3.0f * kTanh1), f2(kTanh0)), p);
+  }
+  const F2 p = sigmoid_exp2(z * f2(-kLog2e));
+  const F2 q = fma2(p, p * f2(-1.0f), p);
+  return fma2(z, q, p);
+}
+
+template <int ACT, int N>
+__device__ __forceinline__ void act_forward_as(float (&v)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; i += 2) split(act_value(f2(v[i], v[i + 1]), ACT), v[i], v[i + 1]);
 }
 
 template <int N>
@@ -181,18 +259,19 @@ __device__ __forceinline__ void act_forward(float (&v)[N], int act) {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = v[i] <= 0.0f ? 0.0f : v[i];
   } else if (act == ACT_GELU) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      float bell;
-      v[i] *= normal_cdf(v[i], bell);
-    }
+    act_forward_as<ACT_GELU>(v);
   } else if (act == ACT_GELU_TANH) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] *= sigmoid(gelu_tanh_2u(v[i]));
+    act_forward_as<ACT_GELU_TANH>(v);
   } else if (act == ACT_SILU) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] *= sigmoid(v[i]);
+    act_forward_as<ACT_SILU>(v);
   }
+}
+
+template <int ACT, int N>
+__device__ __forceinline__ void act_backward_as(float (&v)[N], const float (&z)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; i += 2)
+    split(f2(v[i], v[i + 1]) * act_slope(f2(z[i], z[i + 1]), ACT), v[i], v[i + 1]);
 }
 
 // v[i] *= derivative of the activation at z[i].
@@ -202,25 +281,11 @@ __device__ __forceinline__ void act_backward(float (&v)[N], const float (&z)[N],
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] *= z[i] > 0.0f ? 1.0f : 0.0f;
   } else if (act == ACT_GELU) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      float bell;
-      const float cdf = normal_cdf(z[i], bell);
-      v[i] *= cdf + z[i] * 0.3989422804014327f * bell;
-    }
+    act_backward_as<ACT_GELU>(v, z);
   } else if (act == ACT_GELU_TANH) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      // d(2u)/dz = 2 sqrt(2/pi) (1 + 3 * 0.044715 z^2)
-      const float p = sigmoid(gelu_tanh_2u(z[i]));
-      v[i] *= p + z[i] * p * (1.0f - p) * 1.5957691216057308f * (1.0f + 0.134145f * z[i] * z[i]);
-    }
+    act_backward_as<ACT_GELU_TANH>(v, z);
   } else if (act == ACT_SILU) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float p = sigmoid(z[i]);
-      v[i] *= p * (1.0f + z[i] * (1.0f - p));
-    }
+    act_backward_as<ACT_SILU>(v, z);
   }
 }
 
@@ -887,6 +952,7 @@ struct OuterWalk {
       x.m0 = tm * 256;
       x.n0 = tn * 256 + part * 128;
       if (x.n0 >= g.GN) continue;  // the second half of a tile that has only one
+      if (x.n0 + 128 >= g.GN) x.chunks = 1;
       const int len = C::GROUPED ? tab_off[x.grp + 1] - tab_off[x.grp] : g.GK;
       x.r0 = C::GROUPED ? tab_off[x.grp] : 0;
       // dense: TMA fills the rows behind the last with zeros
@@ -1471,10 +1537,12 @@ __global__ void __launch_bounds__(C::THREADS)
 // slope_kernel
 // ===========================================================================
 // dpre = dout * act'(preact), and/or the column sums of dpre (before its
-// rounding) over all rows.  A block owns 128 columns and every `split`-th
-// block of 16 rows: 16 threads cover a row's 256 bytes.  For the sums the
-// `split` blocks of a column stripe are a cluster: a thread's eight column
-// sums meet in shared memory and then over the cluster, in a fixed order.
+// rounding) over all rows.  A block owns 8 LANES columns and every `split`-th
+// block of rows: LANES threads cover a row's 16 LANES bytes.  For the sums the
+// `split` blocks of a column stripe are a cluster, of at most eight: a
+// thread's eight column sums meet in shared memory and then over the cluster,
+// in a fixed order.  The fewer columns there are, the narrower the stripes, so
+// that the blocks fill the GPU.
 struct SlopeArgs {
   const unsigned short *dout, *preact;
   unsigned short *dpre;
@@ -1484,14 +1552,18 @@ struct SlopeArgs {
   int groups;
 };
 
-constexpr int kSlopeThreads = 256, kSlopeRows = kSlopeThreads / 16;
+constexpr int kSlopeThreads = 256;
 
+// BENT: there is an activation, and dpre is written.
+template <int LANES, bool BENT>
 __global__ void __launch_bounds__(kSlopeThreads, 4) slope_kernel(const SlopeArgs a) {
-  __shared__ float part[kSlopeThreads / 32][128];
+  constexpr int ROWS = kSlopeThreads / LANES, COLS = 8 * LANES;
+  constexpr int U = BENT ? 2 : 4;  // rows in flight per thread: 64 bytes either way
+  __shared__ float part[kSlopeThreads / 32][COLS];
   __shared__ int last;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid % LANES;
   const int stripe = blockIdx.x / a.split, rank = blockIdx.x - stripe * a.split;
-  const int col = stripe * 128 + (tid & 15) * 8;
+  const int col = stripe * COLS + lane * 8;
   pdl_launch_dependents();
   pdl_wait();
   int lo = 0, hi = a.rows;
@@ -1506,9 +1578,8 @@ __global__ void __launch_bounds__(kSlopeThreads, 4) slope_kernel(const SlopeArgs
   }
   float acc[8] = {};
   if (col < a.cols) {
-    constexpr int U = 2;  // rows in flight per thread
-    const int stride = kSlopeRows * a.split;
-    for (int row = lo + rank * kSlopeRows + (tid >> 4); row < hi; row += U * stride) {
+    const int stride = ROWS * a.split;
+    for (int row = lo + rank * ROWS + tid / LANES; row < hi; row += U * stride) {
       uint4 d[U], z[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -1517,7 +1588,7 @@ __global__ void __launch_bounds__(kSlopeThreads, 4) slope_kernel(const SlopeArgs
         d[u] = z[u] = make_uint4(0, 0, 0, 0);
         if (r < hi) {
           d[u] = __ldcs(reinterpret_cast<const uint4 *>(a.dout + off));
-          if (a.preact) z[u] = __ldcs(reinterpret_cast<const uint4 *>(a.preact + off));
+          if (BENT) z[u] = __ldcs(reinterpret_cast<const uint4 *>(a.preact + off));
         }
       }
 #pragma unroll
@@ -1533,23 +1604,25 @@ __global__ void __launch_bounds__(kSlopeThreads, 4) slope_kernel(const SlopeArgs
           y[2 * h] = bf16_lo(zw[h]);
           y[2 * h + 1] = bf16_hi(zw[h]);
         }
-        if (a.preact) act_backward(x, y, a.act);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) acc[i] += x[i];
-        if (a.dpre)
+        if (BENT) {
+          act_backward(x, y, a.act);
           st_global_v4(a.dpre + static_cast<long long>(r) * a.cols + col, pack_bf16x2(x[0], x[1]),
                        pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[i] += x[i];
       }
     }
   }
   if (!a.dbias) return;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], 16);  // the warp's two rows
-    if ((tid & 31) < 16) part[tid >> 5][(tid & 15) * 8 + i] = acc[i];
+#pragma unroll
+    for (int m = LANES; m < 32; m <<= 1) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], m);  // the warp's rows
+    if ((tid & 31) < LANES) part[tid >> 5][lane * 8 + i] = acc[i];
   }
   __syncthreads();
-  if (tid < 128) {
+  if (tid < COLS) {
     float s = 0.0f;
 #pragma unroll
     for (int i = 0; i < kSlopeThreads / 32; ++i) s += part[i][tid];
@@ -1557,10 +1630,10 @@ __global__ void __launch_bounds__(kSlopeThreads, 4) slope_kernel(const SlopeArgs
   }
   __syncthreads();
   if (a.split > 1) cluster_sync();
-  if (rank == 0 && tid < 128) {
+  if (rank == 0 && tid < COLS) {
     float s = part[0][tid];
     for (int c = 1; c < a.split; ++c) s += ld_cluster_f32(mapa_cluster(smem_u32(&part[0][tid]), c));
-    const int n = stripe * 128 + tid;
+    const int n = stripe * COLS + tid;
     if (n < a.cols) a.dbias[n] = s;
   }
   __syncwarp();

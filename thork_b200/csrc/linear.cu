@@ -255,20 +255,32 @@ int weight_gradient(const void *x, const void *dy, int rows, int n, int k, const
   return launch(kern, 2 * pairs, C::THREADS, C::SMEM_BYTES, 2, s, what, tx, ty, tx16, ty16, tout, g);
 }
 
+template <int LANES>
+int run_slope(const SlopeArgs &a, int cluster, cudaStream_t s, const char *what) {
+  const unsigned grid = static_cast<unsigned>(ceil_div(a.cols, 8 * LANES)) * a.split;
+  return a.preact ? launch(slope_kernel<LANES, true>, grid, kSlopeThreads, 0, cluster, s, what, a)
+                  : launch(slope_kernel<LANES, false>, grid, kSlopeThreads, 0, cluster, s, what, a);
+}
+
 int slope(SlopeArgs a, cudaStream_t s, const char *what) {
   int rc, sms;
   if ((rc = thork_sm_count(&sms))) return rc;
-  const long long stripes = (a.cols + 127) / 128;
-  // one wave of four blocks per SM, at most one per 32 rows; the column sums'
-  // blocks are a cluster, of at most eight
-  long long split = 4ll * sms / stripes;
-  if (split < 1) split = 1;
-  const long long most = (a.rows + 31) / 32;
+  const int wave = 4 * sms;  // one wave of four blocks per SM
+  // the widest stripes whose blocks, at most eight a stripe where they are
+  // summed, come near one wave
+  int lanes = 16;
+  while (a.dbias && lanes > 4 && 8ll * ceil_div(a.cols, 8 * lanes) * 4 < 3ll * wave) lanes /= 2;
+  int split = wave / ceil_div(a.cols, 8 * lanes);
+  // no more than leave a block two passes over its rows
+  const int most = ceil_div(a.rows, 2 * kSlopeThreads / lanes);
   if (split > most) split = most;
   if (a.dbias && split > 8) split = 8;
-  a.split = static_cast<int>(split);
-  return launch(slope_kernel, static_cast<unsigned>(stripes * split), kSlopeThreads, 0, a.dbias ? a.split : 1, s, what,
-                a);
+  if (split < 1) split = 1;
+  a.split = split;
+  const int cluster = a.dbias ? split : 1;
+  return lanes == 16 ? run_slope<16>(a, cluster, s, what)
+         : lanes == 8 ? run_slope<8>(a, cluster, s, what)
+                      : run_slope<4>(a, cluster, s, what);
 }
 
 // ---------------------------------------------------------------- checks
