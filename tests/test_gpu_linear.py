@@ -105,6 +105,9 @@ def test_linear_residual_in_place_and_device_arrays(m):
     other.close()  # borrowed: the stream stays usable
     s.synchronize()
     np.testing.assert_array_equal(out.to_host(), want)
+    host = re.copy()
+    f(host, a, b, residual=host)
+    np.testing.assert_array_equal(host, want)
 
 
 @pytest.mark.parametrize("m", [4, 64, 400])
@@ -141,6 +144,34 @@ def test_linear_repeats_bit_for_bit_on_two_streams(m, n, k):
     first = outs[0].to_host()
     for o in outs[1:]:
         np.testing.assert_array_equal(o.to_host(), first)
+
+
+def test_linear_output_past_2_31_elements():
+    """Rows whose elements lie beyond 2^31 (a 4.3 GB output): the first and the
+    last rows against the formula, on the product and on the bias gradient's
+    kernel."""
+    n, k = 14336, 8
+    m = (1 << 31) // n + 200
+    rng = np.random.default_rng(10)
+    a, b = bits(rng, m, k), bits(rng, k, n)
+    A, B, out, dout = rt.to_device(a), rt.to_device(b), rt.empty((m, n), np.uint16), rt.empty((m, n), np.uint16)
+    f = tk.kernels.linear(m, n, k, activation="relu")
+    f(out, A, B, preact=dout)
+
+    def rows(x, r0, r1):
+        got = np.empty((r1 - r0, n), np.uint16)
+        rt.copy_dtoh(got, x.ptr + r0 * n * 2)
+        return got
+
+    for r0, r1 in ((0, 70), (m - 130, m)):
+        z, err = product(wide(a[r0:r1]), wide(b))
+        close(rows(out, r0, r1), np.maximum(z, 0), err, f"rows {r0}..{r1}")
+    # dpre = dout * (preact > 0) with dout = preact is the output again
+    dpre, dbias = rt.empty((m, n), np.uint16), rt.empty((n,), np.float32)
+    tk.kernels.linear_backward(m, n, k, activation="relu")(None, None, dbias, dout, None, None, dout, dpre)
+    for r0, r1 in ((0, 70), (m - 130, m)):
+        np.testing.assert_array_equal(oracle.bf16_bits_to_f32(rows(dpre, r0, r1)),
+                                      oracle.bf16_bits_to_f32(rows(out, r0, r1)))
 
 
 # ---------------------------------------------------------------- backward

@@ -1587,8 +1587,8 @@ __global__ void __launch_bounds__(kSlopeThreads, 4) slope_kernel(const SlopeArgs
         const long long off = static_cast<long long>(r) * a.cols + col;
         d[u] = z[u] = make_uint4(0, 0, 0, 0);
         if (r < hi) {
-          d[u] = __ldcs(reinterpret_cast<const uint4 *>(a.dout + off));
-          if (BENT) z[u] = __ldcs(reinterpret_cast<const uint4 *>(a.preact + off));
+          d[u] = __ldg(reinterpret_cast<const uint4 *>(a.dout + off));
+          if (BENT) z[u] = __ldg(reinterpret_cast<const uint4 *>(a.preact + off));
         }
       }
 #pragma unroll
