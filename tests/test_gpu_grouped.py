@@ -207,6 +207,30 @@ def test_offsets_that_are_wrong_are_clamped_and_reported():
     f(out, a, b, off)
     assert rt.kernel_status() & 0xFF == 2
     np.testing.assert_array_equal(out, want)
+    # the backward pass clamps alike
+    dout = bits(rng, t, n)
+    got = []
+    for o in (off, np.array([0, 10, 10, 40, 40], np.int32)):
+        da, db = np.zeros((t, k), np.uint16), np.zeros((e, k, n), np.uint16)
+        dz, z = np.zeros((t, n), np.uint16), out
+        tk.kernels.grouped_matmul_backward(e, t, n, k, activation="silu")(da, db, dout, a, b, o, z, dz)
+        got.append((da, db, dz))
+        assert rt.kernel_status() & 0xFF == (2 if o is off else 0)
+    for x, y in zip(*got):
+        np.testing.assert_array_equal(x, y)
+
+
+def test_every_row_in_one_group():
+    """The largest group that the buffer allows, with kernels chosen for a few
+    rows a group."""
+    e, t, n, k = 32, 500, 136, 72
+    rng = np.random.default_rng(8)
+    a, b = bits(rng, t, k), bits(rng, e, k, n, std=0.1)
+    for at in (0, 17, 31):
+        off = np.where(np.arange(e + 1) <= at, 0, t).astype(np.int32)
+        out = np.zeros((t, n), np.uint16)
+        tk.kernels.grouped_matmul(e, t, n, k)(out, a, b, off)
+        close(out, *product(wide(a), wide(b[at])), f"group {at}")
 
 
 def test_expert_layers_forward_and_backward():

@@ -74,6 +74,21 @@ def test_operand_checks():
     o.check(d, 1)
     with pytest.raises(ValueError, match="device 1"):
         o.check(d, 0)
+    Elsewhere.ptr = 0
+    with pytest.raises(ValueError, match="freed"):
+        o.check(d, 1)
+
+
+def test_borrowed_streams_stay_their_owners(monkeypatch):
+    destroyed = []
+    monkeypatch.setattr(rt.lib(), "thork_stream_destroy", destroyed.append, raising=False)
+    s = rt.Stream.from_handle(0)
+    assert s.handle is None  # the legacy default stream
+    s.close()
+    s = rt.Stream.from_handle(4096)
+    assert s.handle == 4096
+    s.close()
+    assert s.handle is None and not destroyed
 
 
 def test_c_entry_points_refuse_before_touching_a_device():

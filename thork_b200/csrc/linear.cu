@@ -206,17 +206,19 @@ int dense_product(const Product &p, const GemmArgs &g, cudaStream_t s, const cha
   }
 }
 
-// The groups' sizes are on the device, so the rule goes by their mean.  Few
-// rows a group: swap_kernel, whose tiles waste no instruction on rows that are
-// not there; more: rows_kernel (us, mean rows 2 / 8 / 31 / 63: E=8 of 14336 x
-// 4096 126 against 131 with rows_kernel; E=64 of 2048 x 2048 86 / 85; E=37 of
-// 760 x 1304 28.6 / 22.3; e4m3 E=64 of 2048 x 1024 48 / 35).
+// The groups' sizes are on the device, so the rule goes by their mean and their
+// sum.  Few rows a group: swap_kernel, whose tiles waste no instruction on
+// rows that are not there; more, or so many in all that one group alone may
+// hold many: rows_kernel (us, mean rows 2 / 3 / 8 / 31 / 63: E=8 of 14336 x
+// 4096 126 against 131 with rows_kernel; E=52 of 1432 x 2416 50 / 55; E=64 of
+// 2048 x 2048 86 / 85; E=37 of 760 x 1304 28.6 / 22.3; e4m3 E=64 of 2048 x
+// 1024 48 / 35).
 template <int KIND, bool W_MN>
 int grouped_product(const Product &p, const GemmArgs &g, cudaStream_t s, const char *what) {
   int rc, sms;
   if ((rc = thork_sm_count(&sms))) return rc;
   const int mean = ceil_div(p.rows, p.groups);
-  if (mean > 24) return rows_product<KIND, W_MN, true>(p, g, s, what);
+  if (mean > 24 || p.rows > 512) return rows_product<KIND, W_MN, true>(p, g, s, what);
   // two CTAs fit on an SM: split the contraction until they are all in use
   const long long held = p.groups < p.rows ? p.groups : p.rows;
   const int nkb = ceil_div(p.k, KIND == KIND_BF16 ? 64 : 128);

@@ -116,6 +116,8 @@ class Operand:
         if host:
             if not a.flags["C_CONTIGUOUS"]:
                 raise ValueError(f"Argument for '{self.name}' must be C-contiguous")
+        elif not a.buffer.ptr:
+            raise ValueError(f"Argument for '{self.name}' is an array that has been freed")
         elif a.buffer._dev != dev:
             raise ValueError(f"Argument for '{self.name}' is on device {a.buffer._dev}; the call runs on "
                              f"device {dev}")
@@ -138,9 +140,10 @@ def run_operands(operands: Sequence[Operand], args: Sequence, launch: Callable, 
             # the checks of an array that passes them, in line: a call's host
             # time shows when its kernel takes a few microseconds
             if type(a) is DeviceArray:
-                if a.dtype is not o.seen or a.size != o.count or a.buffer._dev != dev:
+                buf = a.buffer
+                if a.dtype is not o.seen or a.size != o.count or buf._dev != dev or not buf.ptr:
                     o.check(a, dev)
-                ptrs.append(a.buffer.ptr)
+                ptrs.append(buf.ptr)
                 continue
             o.check(a, dev)
             if isinstance(a, DeviceArray):

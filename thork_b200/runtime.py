@@ -453,8 +453,8 @@ def wrap_pointer(ptr: int, shape, dtype, owner=None) -> DeviceArray:
     """A DeviceArray over C-contiguous device memory of another library, on
     the current device (for example a torch tensor's ``data_ptr()``, with the
     tensor as ``owner`` so that it outlives the array)."""
-    n = int(np.prod(shape, dtype=np.int64)) * np.dtype(dtype).itemsize
-    return DeviceArray(shape, dtype, buffer=_Borrowed(ptr, n, owner))
+    dtype = np.dtype(dtype)
+    return DeviceArray(shape, dtype, buffer=_Borrowed(ptr, math.prod(shape) * dtype.itemsize, owner))
 
 
 def copy_htod(d_ptr: int, arr: np.ndarray, stream: Optional[Stream] = None, sync: bool = True) -> None:
