@@ -210,7 +210,8 @@ def test_linear_backward_activations(activation):
 
 @pytest.mark.parametrize("m,n,k", [(1, 8, 8), (1, 256, 512), (13, 136, 264), (40, 1024, 128),
                                    (100, 520, 1032), (128, 64, 64), (257, 328, 264), (1000, 776, 520),
-                                   (2500, 136, 2304), (640, 2304, 2304)])
+                                   (2500, 136, 2304), (640, 2304, 2304), (2604, 184, 152), (3001, 520, 264),
+                                   (4100, 72, 1000), (6000, 1032, 520)])
 def test_linear_backward_shapes(m, n, k):
     _backward(m, n, k, "silu", seed=1)
     _backward(m, n, k, "none", seed=2)

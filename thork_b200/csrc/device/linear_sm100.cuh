@@ -1286,10 +1286,14 @@ __global__ void __launch_bounds__(C::THREADS, 1)
 // fp32 accumulators go to their own shared memory, [row][128] floats over the
 // finished pipeline stages, and each CTA sums every S-th row over the cluster
 // in rank order (deterministic, no workspace in global memory) and stores it.
-template <int KIND_, int BN_, int STAGES_, bool W_MN_, bool GROUPED_>
+//
+// X_MN: X is given as its transpose, [k, m] row-major.  That is the weights'
+// gradient, out[k, n] = sum over rows X[row, k] dY[row, n], where it has few
+// tiles and many rows to sum over.
+template <int KIND_, int BN_, int STAGES_, bool W_MN_, bool X_MN_, bool GROUPED_>
 struct SwapCfg {
   static constexpr int KIND = KIND_, BN = BN_, STAGES = STAGES_;
-  static constexpr bool W_MN = W_MN_, GROUPED = GROUPED_;
+  static constexpr bool W_MN = W_MN_, X_MN = X_MN_, GROUPED = GROUPED_;
   static constexpr int ELEM = KIND == KIND_BF16 ? 2 : 1;
   static constexpr int BM = 128;
   static constexpr int BK = 128 / ELEM;
@@ -1305,7 +1309,8 @@ struct SwapCfg {
   static constexpr int TAB_BYTES = GROUPED ? (kMaxGroups + 1) * 8 : 0;
   static constexpr int SMEM_BYTES = 1024 + TAB_OFF + TAB_BYTES;
   static constexpr u32 IDESC =
-      make_idesc(KIND == KIND_BF16 ? 1u : 0u, KIND == KIND_BF16 ? 1u : 0u, W_MN, false, BM, BN);
+      make_idesc(KIND == KIND_BF16 ? 1u : 0u, KIND == KIND_BF16 ? 1u : 0u, W_MN, X_MN, BM, BN);
+  static_assert(!X_MN || BN % CHUNK == 0, "an MN-major operand is whole 128-byte lines");
   static_assert(BN * BM * 4 <= STAGES * STAGE_BYTES, "the fp32 tile overlays the stages");
   static_assert(BN % 16 == 0 && BN <= 128, "tile rows");
   // two CTAs share an SM; a third never does (tensor memory: 3 x 128 columns would still fit)
@@ -1407,7 +1412,7 @@ __global__ void __launch_bounds__(C::THREADS)
             load_w(pre, kb0 + pre);
           }
         }
-        pdl_wait();
+        if (!g.wait_last) pdl_wait();
         if (g.trigger_late) pdl_launch_dependents();
         int s = 0;
         u32 ph = 0;
@@ -1417,7 +1422,14 @@ __global__ void __launch_bounds__(C::THREADS)
             mbar_arrive_expect_tx(full_bar(s), C::STAGE_BYTES);
             load_w(s, kb);
           }
-          tma_load_3d(base + s * C::STAGE_BYTES + C::W_BYTES, &tmap_x, full_bar(s), kb * C::BK, m0, 0);
+          const u32 sx = base + s * C::STAGE_BYTES + C::W_BYTES;
+          if (C::X_MN) {
+#pragma unroll
+            for (int c = 0; c < C::BN / C::CHUNK; ++c)
+              tma_load_3d(sx + c * C::BK * 128, &tmap_x, full_bar(s), m0 + c * C::CHUNK, kb * C::BK, 0);
+          } else {
+            tma_load_3d(sx, &tmap_x, full_bar(s), kb * C::BK, m0, 0);
+          }
           if (++s == C::STAGES) {
             s = 0;
             ph ^= 1u;
@@ -1436,7 +1448,8 @@ __global__ void __launch_bounds__(C::THREADS)
           for (int k = 0; k < C::BK / C::UMMA_K; ++k) {
             const u64 ad = C::W_MN ? smem_desc_sw128(sw + k * C::UMMA_K * 128, C::BK * 128, 1024)
                                    : smem_desc_sw128(sw + k * 32, 16, 1024);
-            const u64 bd = smem_desc_sw128(sx + k * 32, 16, 1024);
+            const u64 bd = C::X_MN ? smem_desc_sw128(sx + k * C::UMMA_K * 128, C::BK * 128, 1024)
+                                   : smem_desc_sw128(sx + k * 32, 16, 1024);
             const u32 accum = (kb > kb0 || k > 0) ? 1u : 0u;
             if (C::KIND == KIND_BF16)
               mma_f16_ss(tmem_base, ad, bd, C::IDESC, accum);
@@ -1452,7 +1465,7 @@ __global__ void __launch_bounds__(C::THREADS)
         tc_commit(done_bar);
       }
     } else {
-      pdl_wait();  // bias, residual and outputs are ordered after the previous kernel
+      if (!g.wait_last) pdl_wait();  // bias, residual and outputs are ordered after the previous kernel
       const int q = warp & 3;
       bool ok = true;
       if (lane == 0) ok = mbar_wait(done_bar, 0, status, 0x53);
@@ -1462,13 +1475,17 @@ __global__ void __launch_bounds__(C::THREADS)
         // every load has landed and been read: the stages are free
         float *acc = reinterpret_cast<float *>(smem) + q * 32 + lane;
         const u32 t_row = tmem_base + (static_cast<u32>(q * 32) << 16);
+        constexpr int CH = C::BN < 32 ? 16 : 32;
 #pragma unroll 1
-        for (int r0 = 0; r0 < rows; r0 += 16) {
-          u32 r[16];
-          tmem_ld_32x32b_x16(t_row + r0, r);
+        for (int r0 = 0; r0 < rows; r0 += CH) {
+          u32 r[CH];
+          if constexpr (CH == 32)
+            tmem_ld_32x32b_x32(t_row + r0, r);
+          else
+            tmem_ld_32x32b_x16(t_row + r0, r);
           tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
+          for (int i = 0; i < CH; ++i)
             if (r0 + i < rows) acc[(r0 + i) * C::BM] = __uint_as_float(r[i]);
         }
       }
@@ -1530,6 +1547,7 @@ __global__ void __launch_bounds__(C::THREADS)
   }
   __syncthreads();
   tc_fence_after();
+  if (g.wait_last) pdl_wait();
   if (warp == 1) tmem_dealloc<1>(tmem_base, C::TMEM_COLS);
 }
 

@@ -101,7 +101,7 @@ int map_x(TensorMap &t, const Product &p, int box_rows) {
 
 template <int KIND, int BN, int STAGES, bool W_MN, bool GROUPED>
 int swap_product(const Product &p, const GemmArgs &g, int split, cudaStream_t s, const char *what) {
-  using C = SwapCfg<KIND, BN, STAGES, W_MN, GROUPED>;
+  using C = SwapCfg<KIND, BN, STAGES, W_MN, false, GROUPED>;
   int rc;
   alignas(64) TensorMap tw, tx;
   if ((rc = map_w<KIND, W_MN>(tw, p, C::BM))) return rc;
@@ -228,6 +228,21 @@ int grouped_product(const Product &p, const GemmArgs &g, cudaStream_t s, const c
   return swap_product<KIND, 32, 5, W_MN, true>(p, g, split, s, what);
 }
 
+// The dense weight gradient by swap_kernel: 128 columns n by BN rows k a
+// cluster, the rows of X and dY split over it.
+template <int BN, int STAGES>
+int swap_gradient(const void *x, const void *dy, int rows, int n, int k, const GemmArgs &args, int split,
+                  cudaStream_t s, const char *what) {
+  using C = SwapCfg<KIND_BF16, BN, STAGES, true, true, false>;
+  int rc;
+  alignas(64) TensorMap tx, ty;
+  if ((rc = thork_encode_tmap_3d(&ty, THORK_DT_BF16, dy, n, rows, 1, C::CHUNK, C::BK))) return rc;
+  if ((rc = thork_encode_tmap_3d(&tx, THORK_DT_BF16, x, k, rows, 1, C::CHUNK, C::BK))) return rc;
+  GemmArgs g = args;
+  g.w_static = 0;
+  return run_swap<C>(ty, tx, g, static_cast<long long>(ceil_div(k, BN)) * ceil_div(n, C::BM), split, s, what);
+}
+
 // dW[k, n] = sum over rows X[m, k] dY[m, n], of each group's rows when grouped.
 template <bool GROUPED>
 int weight_gradient(const void *x, const void *dy, int rows, int n, int k, const GemmArgs &g,
@@ -255,6 +270,32 @@ int weight_gradient(const void *x, const void *dy, int rows, int n, int k, const
   const long long most = 2ll * ((k + 255) / 256) * ((n + 255) / 256) * (GROUPED ? g.groups : 1);
   const int pairs = static_cast<int>(most < sms / 2 ? most : sms / 2);
   return launch(kern, 2 * pairs, C::THREADS, C::SMEM_BYTES, 2, s, what, tx, ty, tx16, ty16, tout, g);
+}
+
+// Few tiles with many rows to sum over: split the rows over clusters, by the
+// estimates of dense_product (us, outer_kernel / swap_kernel: 2604 rows of 184
+// x 152 17.0 / 7.7, 8054 of 256 x 536 32.3 / 12.6, 8192 of 1024 x 1024 30.9 /
+// 22.7; 637 of 1800 x 488 8.5 / 10.7, 7008 of 2168 x 1384 53 / 96).
+int dense_gradient(const void *x, const void *dy, int rows, int n, int k, const GemmArgs &g, cudaStream_t s,
+                   const char *what) {
+  int rc, sms;
+  if ((rc = thork_sm_count(&sms))) return rc;
+  const int nkb = ceil_div(rows, 64);
+  const double mbytes = 2e-6 * (static_cast<double>(n) * k + static_cast<double>(rows) * (n + k));
+  double best = rows_us(nkb, k, n, mbytes, sms / 2);
+  int bn = 0, split = 0;
+  for (int b = 64; b <= 128; b *= 2)
+    for (int c = 1; c <= 8 && 2 * c <= nkb + 1; c *= 2) {
+      const double us = swap_us(nkb, k, n, mbytes, sms, b, c);
+      if (us < best) {
+        best = us;
+        bn = b;
+        split = c;
+      }
+    }
+  if (bn == 64) return swap_gradient<64, 4>(x, dy, rows, n, k, g, split, s, what);
+  if (bn == 128) return swap_gradient<128, 3>(x, dy, rows, n, k, g, split, s, what);
+  return weight_gradient<false>(x, dy, rows, n, k, g, s, what);
 }
 
 template <int LANES>
@@ -436,7 +477,7 @@ int backward(void *da, void *db, float *dbias, const void *dout, const void *a, 
     w.GK = rows;
     w.wait_last = da != nullptr;
     rc = groups ? weight_gradient<true>(a, dz, rows, N, K, w, s, what)
-                : weight_gradient<false>(a, dz, rows, N, K, w, s, what);
+                : dense_gradient(a, dz, rows, N, K, w, s, what);
     if (rc) return rc;
   }
   return THORK_OK;
