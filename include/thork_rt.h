@@ -327,10 +327,11 @@ THORK_API int thork_skinny_gemm_bf16_noalloc_status(unsigned *status, int clear,
  * gradients.  No reference counterpart (its tk.kernels.matmul is a plain
  * product, src/thork/kernels/matmul.py:17-71).  All queue work on `stream`
  * and return without synchronising; none allocates or keeps a workspace
- * (the status word is allocated by the first call on a device, so make one
- * call before a stream capture).  Arrays are dense row-major device memory,
- * 16-byte aligned; bf16 unless said otherwise.  Sums are fp32; every output
- * is rounded once.                                                         */
+ * (the status word is allocated by the first call on a device, and a kernel
+ * is loaded by its first, so make one call of the same sizes before a stream
+ * capture).  Arrays are dense row-major device memory,
+ * 16-byte aligned; bf16 unless said otherwise; sizes are at most 2^30.  Sums
+ * are fp32; every output is rounded once.                                  */
 enum {
   THORK_ACT_NONE = 0,
   THORK_ACT_RELU = 1,

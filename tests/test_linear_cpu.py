@@ -14,7 +14,7 @@ K = tk.kernels
 @pytest.mark.parametrize("make", [
     lambda: K.linear(0, 64, 64), lambda: K.linear(4, 60, 64), lambda: K.linear(4, 64, 20),
     lambda: K.linear(4, 72, 64, tk.dt.float8_e4m3), lambda: K.linear(4, 64, 64, activation="tanh"),
-    lambda: K.linear(1 << 31, 64, 64), lambda: K.linear_backward(-1, 64, 64),
+    lambda: K.linear((1 << 30) + 1, 64, 64), lambda: K.linear_backward(-1, 64, 64),
     lambda: K.linear_backward(4, 64, 12), lambda: K.grouped_matmul(0, 4, 64, 64),
     lambda: K.grouped_matmul(1025, 4, 64, 64), lambda: K.grouped_matmul(2, 0, 64, 64),
     lambda: K.grouped_matmul(2, 4, 64, 72, tk.dt.float8_e4m3),
@@ -107,6 +107,7 @@ def test_c_entry_points_refuse_before_touching_a_device():
     bad(lin(16, 32, 48, None, 64, 64, 4, 64, 64, 0, 0, None), "same array")
     bad(lin(16, 32, 48, None, None, None, 4, 60, 64, 0, 0, None), "multiples of 8")
     bad(lin(16, 32, 48, None, None, None, 0, 64, 64, 0, 0, None), "positive")
+    bad(lin(16, 32, 48, None, None, None, (1 << 30) + 1, 64, 64, 0, 0, None), "at most 2^30")
     bad(lin(16, 32, 48, None, None, None, 4, 64, 64, 5, 0, None), "activation")
     bad(lin(16, 32, 48, None, None, None, 4, 64, 64, 0, 2, None), "flags")
     bad(L.thork_linear_e4m3(16, 32, 48, None, None, None, 4, 72, 64, 1.0, 1.0, 0, 0, None), "multiples of 16")

@@ -30,6 +30,12 @@ enum : int { ACT_NONE = 0, ACT_RELU = 1, ACT_GELU = 2, ACT_GELU_TANH = 3, ACT_SI
 
 constexpr int kMaxGroups = 1024;
 
+// Every kernel here may start before the kernel that writes its inputs has
+// ended (programmatic dependent launch), and out may be the residual itself.
+// So ordinary loads go past L1 (ld.global.cg): neither a read-only load, whose
+// data may not change while the kernel lives, nor a line that this SM cached
+// before the wait can return an old value.
+
 // What happens to an accumulator on its way to the output:
 //   z = acc * alpha [* group_scale[g]] + bias;  preact = z;
 //   out = act(z) + residual
@@ -300,7 +306,7 @@ __device__ __forceinline__ void scan_groups(const int *offsets, int groups, int 
   bool bad = false;
   for (int base = 0; base <= groups; base += 32) {
     const int i = base + lane;
-    const int raw = i <= groups ? offsets[i] : 0;
+    const int raw = i <= groups ? __ldcg(offsets + i) : 0;
     int v = max(0, min(raw, rows));
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -562,9 +568,8 @@ __device__ __forceinline__ void load_block(uint4 (&v)[4], const unsigned short *
   for (int it = 0; it < 4; ++it) {
     const int row = row0 + 8 * it + (lane >> 2);
     v[it] = make_uint4(0, 0, 0, 0);
-    // an ordinary load: out may be the residual itself
     if (row < row_end && col < cols)
-      v[it] = *reinterpret_cast<const uint4 *>(src + static_cast<long long>(row) * cols + col);
+      v[it] = __ldcg(reinterpret_cast<const uint4 *>(src + static_cast<long long>(row) * cols + col));
   }
 }
 
@@ -769,7 +774,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     RowTile x;
     int it = 0;
     while (!*abort_flag && walk.next(x)) {
-      const float alpha = p.group_scale ? p.alpha * __ldg(p.group_scale + x.grp) : p.alpha;
+      const float alpha = p.group_scale ? p.alpha * __ldcg(p.group_scale + x.grp) : p.alpha;
       const int col0 = x.n0 + rank * C::BNC + q * 32;  // the warp's columns, one per lane
       const bool live = col0 < p.cols;
       float bias[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // of columns lane / 4 + 8 i
@@ -777,7 +782,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int col = col0 + 8 * i + (lane >> 2);
-          if (col < p.cols) bias[i] = __uint_as_float(static_cast<u32>(p.bias[col]) << 16);
+          if (col < p.cols) bias[i] = __uint_as_float(static_cast<u32>(__ldcg(p.bias + col)) << 16);
         }
       }
       uint4 res[4];
@@ -1500,17 +1505,17 @@ __global__ void __launch_bounds__(C::THREADS)
     if (warp >= 2) {
       const Epilogue &p = g.epi;
       const int col = n0 + 4 * lane;
-      const float alpha = p.group_scale ? p.alpha * __ldg(p.group_scale + grp) : p.alpha;
+      const float alpha = p.group_scale ? p.alpha * __ldcg(p.group_scale + grp) : p.alpha;
       float4 bias = make_float4(0.f, 0.f, 0.f, 0.f);
       if (p.bias && col < p.cols) {
-        const uint2 w = __ldg(reinterpret_cast<const uint2 *>(p.bias + col));
+        const uint2 w = __ldcg(reinterpret_cast<const uint2 *>(p.bias + col));
         bias = make_float4(bf16_lo(w.x), bf16_hi(w.x), bf16_lo(w.y), bf16_hi(w.y));
       }
       for (int r = rank + S * (warp - 2); r < rows; r += 4 * S) {
         const long long off = static_cast<long long>(m0 + r) * p.cols + col;
         const u32 at = base + (r * C::BM + 4 * lane) * 4;
         uint2 res = make_uint2(0, 0);
-        if (p.residual && col < p.cols) res = *reinterpret_cast<const uint2 *>(p.residual + off);
+        if (p.residual && col < p.cols) res = __ldcg(reinterpret_cast<const uint2 *>(p.residual + off));
         float v[4] = {0.f, 0.f, 0.f, 0.f};
         if (S > 1) {
           for (int c = 0; c < S; ++c) {
@@ -1589,9 +1594,9 @@ __global__ void __launch_bounds__(kSlopeThreads, 4) slope_kernel(const SlopeArgs
     // the last group ends at the largest clamped offset
     if (tid == 0) last = 0;
     __syncthreads();
-    for (int i = tid; i <= a.groups; i += kSlopeThreads) atomicMax(&last, min(a.offsets[i], a.rows));
+    for (int i = tid; i <= a.groups; i += kSlopeThreads) atomicMax(&last, min(__ldcg(a.offsets + i), a.rows));
     __syncthreads();
-    lo = max(0, min(a.offsets[0], a.rows));
+    lo = max(0, min(__ldcg(a.offsets), a.rows));
     hi = last;
   }
   float acc[8] = {};
@@ -1605,8 +1610,8 @@ __global__ void __launch_bounds__(kSlopeThreads, 4) slope_kernel(const SlopeArgs
         const long long off = static_cast<long long>(r) * a.cols + col;
         d[u] = z[u] = make_uint4(0, 0, 0, 0);
         if (r < hi) {
-          d[u] = __ldg(reinterpret_cast<const uint4 *>(a.dout + off));
-          if (BENT) z[u] = __ldg(reinterpret_cast<const uint4 *>(a.preact + off));
+          d[u] = __ldcg(reinterpret_cast<const uint4 *>(a.dout + off));
+          if (BENT) z[u] = __ldcg(reinterpret_cast<const uint4 *>(a.preact + off));
         }
       }
 #pragma unroll

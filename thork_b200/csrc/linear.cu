@@ -327,9 +327,15 @@ int slope(SlopeArgs a, cudaStream_t s, const char *what) {
 }
 
 // ---------------------------------------------------------------- checks
+// Row and column numbers, rounded up to whole tiles and passes, are ints.
+constexpr int kMaxDim = 1 << 30;
+
 int check_sizes(int rows, int n, int k, int align, const char *what) {
   if (rows <= 0 || n <= 0 || k <= 0)
     return thork_set_error(THORK_ERR_INVALID, "%s: dimensions must be positive (M=%d N=%d K=%d)", what,
+                           rows, n, k);
+  if (rows > kMaxDim || n > kMaxDim || k > kMaxDim)
+    return thork_set_error(THORK_ERR_INVALID, "%s: dimensions must be at most 2^30 (M=%d N=%d K=%d)", what,
                            rows, n, k);
   if (n % align || k % align)
     return thork_set_error(THORK_ERR_INVALID,

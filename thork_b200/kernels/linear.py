@@ -24,8 +24,8 @@ def activation_code(activation: str, what: str) -> int:
 
 def check_sizes(what: str, dtype: dt.Dtype, N: int, K: int, **positive) -> None:
     for name, v in {**positive, "N": N, "K": K}.items():
-        if not 0 < v < 1 << 31:
-            raise ValueError(f"{what}: {name}={v} must be positive and below 2^31")
+        if not 0 < v <= 1 << 30:
+            raise ValueError(f"{what}: {name}={v} must be positive and at most 2^30")
     align = {dt.bfloat16: 8, dt.float8_e4m3: 16}.get(dtype)
     if align is None:
         raise TypeError(f"{what}: unsupported dtype {dtype!r}")
