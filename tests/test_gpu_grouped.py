@@ -269,3 +269,39 @@ def test_expert_layers_forward_and_backward():
         close(dz.to_host()[r], DH * slope(zb, "silu"), np.abs(DH) * slope_err(zb), "dz")
         close(dx.to_host()[r], *product(DZ, wide(w1[i]).T), "dx")
         close(dw1.to_host()[i], *product(wide(x[r]).T, DZ), "dw1")
+
+
+@pytest.mark.parametrize("sizes", [[2, 0, 1, 5], [30, 0, 100, 7, 260], [1, 16, 17, 300, 0, 64]])
+def test_long_chains_without_a_wait_repeat_those_with_one(sizes):
+    """Layers of experts forward and backward, queued without a wait, against
+    the same calls one by one, bit for bit (see the dense form)."""
+    off = sizes_to_offsets(sizes)
+    e, t, d, f = len(sizes), int(off[-1]), 264, 392
+    rng = np.random.default_rng(13)
+    w1, w2 = rt.to_device(bits(rng, e, d, f, std=0.06)), rt.to_device(bits(rng, e, f, d, std=0.05))
+    o = rt.to_device(off)
+    x0, dy0 = bits(rng, t, d), bits(rng, t, d, std=0.1)
+    K = tk.kernels
+    up, down = K.grouped_matmul(e, t, f, d, activation="gelu"), K.grouped_matmul(e, t, d, f)
+    up_b = K.grouped_matmul_backward(e, t, f, d, activation="gelu")
+    down_b = K.grouped_matmul_backward(e, t, d, f)
+    s = rt.Stream()
+
+    def chain(sync):
+        x, y, dy = rt.to_device(x0), rt.empty((t, d), np.uint16), rt.to_device(dy0)
+        h, z, dz, dh = (rt.empty((t, f), np.uint16) for _ in range(4))
+        dx, dw1, dw2 = rt.empty((t, d), np.uint16), rt.empty((e, d, f), np.uint16), rt.empty((e, f, d), np.uint16)
+        kw = dict(stream=s, sync=sync)
+        for _ in range(8):
+            up(h, x, w1, o, preact=z, **kw)
+            down(y, h, w2, o, **kw)
+            down_b(dh, dw2, dy, h, w2, o, **kw)
+            up_b(dx, dw1, dh, x, w1, o, z, dz, **kw)
+            x, y, dy, dx = y, x, dx, dy
+        s.synchronize()
+        return [v.to_host() for v in (x, dy, h, z, dz, dh, dw1, dw2)]
+
+    want = chain(True)
+    for _ in range(3):
+        for a, b in zip(chain(False), want):
+            np.testing.assert_array_equal(a, b)

@@ -302,3 +302,43 @@ def test_training_step_of_two_layers():
     close(dw1.to_host(), *product(wide(x).T, DZ), "dw1")
     assert np.abs(db1.to_host() - gz.sum(0)).max() <= 1e-4
     assert np.abs(db2.to_host() - wide(dy).sum(0)).max() <= 1e-4
+
+
+@pytest.mark.parametrize("t,d,f", [(8, 264, 520), (160, 136, 392), (700, 520, 1032)])
+def test_long_chains_without_a_wait_repeat_those_with_one(t, d, f):
+    """Twelve layers forward (the residual updated in place) and backward, each
+    call's inputs written by the call before it and its outputs read by the
+    next: queued without a wait, every array is bit for bit what the same calls
+    give one by one.  The kernels of a stream overlap, so a missing wait for the
+    previous kernel would show here."""
+    rng = np.random.default_rng(12)
+    layers = 12
+    w1 = [rt.to_device(bits(rng, d, f, std=0.06)) for _ in range(3)]
+    w2 = [rt.to_device(bits(rng, f, d, std=0.03)) for _ in range(3)]
+    x0, dy0 = bits(rng, t, d), bits(rng, t, d, std=0.1)
+    L = tk.kernels
+    up, down = L.linear(t, f, d, activation="silu", static_weights=True), L.linear(t, d, f, static_weights=True)
+    up_b, down_b = L.linear_backward(t, f, d, activation="silu"), L.linear_backward(t, d, f)
+    s = rt.Stream()
+
+    def chain(sync):
+        x, dy = rt.to_device(x0), rt.to_device(dy0)
+        h, z, dz, dh = (rt.empty((t, f), np.uint16) for _ in range(4))
+        dx, dw1, dw2, db = (rt.empty((t, d), np.uint16), rt.empty((d, f), np.uint16),
+                            rt.empty((f, d), np.uint16), rt.empty((f,), np.float32))
+        kw = dict(stream=s, sync=sync)
+        seen = []
+        for i in range(layers):
+            up(h, x, w1[i % 3], preact=z, **kw)
+            down(x, h, w2[i % 3], residual=x, **kw)
+            down_b(dh, dw2, None, dy, h, w2[i % 3], **kw)
+            up_b(dx, dw1, db, dh, x, w1[i % 3], z, dz, **kw)
+            dy, dx = dx, dy
+        s.synchronize()
+        seen += [v.to_host() for v in (x, dy, h, z, dz, dh, dw1, dw2, db)]
+        return seen
+
+    want = chain(True)
+    for _ in range(3):
+        for a, b in zip(chain(False), want):
+            np.testing.assert_array_equal(a, b)
