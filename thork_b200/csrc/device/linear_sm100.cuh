@@ -158,8 +158,8 @@ __device__ __forceinline__ float bf16_hi(u32 w) { return __uint_as_float(w & 0xF
 //
 // Two values at a time, in the packed fp32 instructions: slope_kernel has
 // about as many instructions to issue as bytes to move (4096 x 14336, gelu:
-// 126 us with erff and expf, 73 with the approximation, 66 packed; its traffic
-// takes 54).
+// 126 us with erff and expf, 73 with the approximation, 65-70 packed; its
+// traffic takes 54).
 struct F2 {
   u64 v;
 };
@@ -354,6 +354,13 @@ __device__ __forceinline__ void scan_groups(const int *offsets, int groups, int 
 //
 // Warps: 0 TMA producer, 1 MMA issuer (leader only), 2..9 epilogue: two warps
 // per TMEM lane quadrant, taking the tile's 32-row slices in turn.
+//
+// Bound by the tensor pipe (90 % of active cycles at 4096 x 4096 x 14336), and
+// back to back by the power cap.  Measured: 4096^3 91 us (1508 TFLOP/s), 8192^3
+// 695 us (1583) in bursts, 832 us (1322) over 1.5 s; e4m3 8192^3 334 us alone;
+// 8 experts of 14336 x 4096 with 8192 rows 651 us alone (1478).  Six stages of
+// 32 KiB per CTA; 512-column tiles of four 48 KiB stages gained 1 % at 8192^3
+// and lost 3 % at 4096^3.
 template <int KIND_, bool W_MN_, bool GROUPED_>
 struct RowsCfg {
   static constexpr int KIND = KIND_, STAGES = 6;
@@ -877,6 +884,11 @@ __global__ void __launch_bounds__(C::THREADS, 1)
 //
 // A warp's 32 rows x 64 columns of the result leave through shared memory by
 // TMA, in whole 128-byte lines; it clips what lies outside dW.
+//
+// Bound by the tensor pipe for many rows (4096 x 4096 x 14336: 95 % of active
+// cycles, 311 us, 1545 TFLOP/s), by the operands' latency for groups of a few
+// hundred (8 x 512 rows of 4096 x 4096: 119 us) and by the writes of dW below
+// (64 x 64 rows of 4096 x 1024: 114 us, 4.7 TB/s; 16-byte stores took 286).
 template <bool GROUPED_>
 struct OuterCfg {
   static constexpr bool GROUPED = GROUPED_;
@@ -1292,6 +1304,10 @@ __global__ void __launch_bounds__(C::THREADS, 1)
 // finished pipeline stages, and each CTA sums every S-th row over the cluster
 // in rank order (deterministic, no workspace in global memory) and stores it.
 //
+// Bound by the weights' bytes: 1 x 14336 x 4096 20.8 us (5.6 TB/s, S=2), 16 x
+// 4096 x 14336 21.5 us (5.5 TB/s, S=8); 128 x 4096 x 4096 14.7 us.  5 to 6
+// stages leave room for two CTAs an SM and hold 190 KiB of loads in flight.
+//
 // X_MN: X is given as its transpose, [k, m] row-major.  That is the weights'
 // gradient, out[k, n] = sum over rows X[row, k] dY[row, n], where it has few
 // tiles and many rows to sum over.
@@ -1440,6 +1456,14 @@ __global__ void __launch_bounds__(C::THREADS)
             ph ^= 1u;
           }
         }
+        // drain: every issued load has landed and been read before the CTA exits
+        for (int i = 0; i < C::STAGES; ++i) {
+          if (!mbar_wait(empty_bar(s), ph ^ 1u, status, 0x54)) break;
+          if (++s == C::STAGES) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
       }
     } else if (warp == 1) {
       if (elect_one()) {
@@ -1566,6 +1590,10 @@ __global__ void __launch_bounds__(C::THREADS)
 // thread's eight column sums meet in shared memory and then over the cluster,
 // in a fixed order.  The fewer columns there are, the narrower the stripes, so
 // that the blocks fill the GPU.
+//
+// Bound by its traffic, with about as many instructions to issue: 4096 x 14336
+// with gelu and the sums 65-70 us (5.0-5.4 TB/s), 4096 x 4096 with silu 17 us
+// (5.9 TB/s).
 struct SlopeArgs {
   const unsigned short *dout, *preact;
   unsigned short *dpre;
