@@ -1,0 +1,57 @@
+"""GPU: calls of the linear-layer operators in unusual company: slow kernels
+before them, status words, extreme values (tolerances derived in
+linear_ref.py)."""
+
+import ctypes
+
+import numpy as np
+import pytest
+
+import thork_b200 as tk
+from linear_ref import act, act_err, bits, close, product, wide
+
+pytestmark = pytest.mark.gpu
+rt = tk.runtime
+
+
+@pytest.fixture(autouse=True)
+def _status():
+    yield
+    assert rt.kernel_status() == 0
+
+
+# Lets its successor start at once and then takes `ns` nanoseconds, as a
+# barrier between GPUs does while a peer is late.  The loop ends by count too.
+SLOW = """
+extern "C" __global__ void slow(unsigned long long ns) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  unsigned long long t0, t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
+  for (int i = 0; i < 40000; ++i) {
+    __nanosleep(100000);
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    if (t - t0 > ns) break;
+  }
+}
+"""
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 256, 512), (5, 264, 2056), (48, 512, 1024)])
+def test_a_product_behind_a_slow_kernel_waits_for_it(m, n, k):
+    """A product of few rows starts beside the kernel before it; its one-second
+    limit must not count the time that that kernel takes (1.4 s here)."""
+    rng = np.random.default_rng(1)
+    a, b = bits(rng, m, k), bits(rng, k, n, std=0.05)
+    A, B, out = rt.to_device(a), rt.to_device(b), rt.empty((m, n), np.uint16)
+    out.zero()
+    f = tk.kernels.linear(m, n, k, activation="silu", static_weights=True)
+    s = rt.Stream()
+    f(out, A, B, stream=s)  # the kernels are loaded
+    out.zero(s)
+    slow = rt.compile_source(SLOW).function("slow")
+    rt.launch(slow, (1, 1, 1), (32, 1, 1), [ctypes.c_ulonglong(1_400_000_000)], stream=s)
+    f(out, A, B, stream=s, sync=False)
+    s.synchronize()
+    assert rt.kernel_status() == 0
+    z, err = product(wide(a), wide(b))
+    close(out.to_host(), act(z, "silu"), act_err(z, err), "out")

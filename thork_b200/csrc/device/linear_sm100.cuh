@@ -145,6 +145,10 @@ __device__ __forceinline__ float ld_cluster_f32(u32 addr) {
   return v;
 }
 
+__device__ __forceinline__ void st_cluster_u32(u32 addr, u32 v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+
 __device__ __forceinline__ float bf16_lo(u32 w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf16_hi(u32 w) { return __uint_as_float(w & 0xFFFF0000u); }
 
@@ -1311,6 +1315,9 @@ __global__ void __launch_bounds__(C::THREADS, 1)
 // X_MN: X is given as its transpose, [k, m] row-major.  That is the weights'
 // gradient, out[k, n] = sum over rows X[row, k] dY[row, n], where it has few
 // tiles and many rows to sum over.
+//
+// A wait that expires in one CTA (an accumulator that is not complete) is told
+// to the whole cluster, which then stores nothing.
 template <int KIND_, int BN_, int STAGES_, bool W_MN_, bool X_MN_, bool GROUPED_>
 struct SwapCfg {
   static constexpr int KIND = KIND_, BN = BN_, STAGES = STAGES_;
@@ -1351,6 +1358,7 @@ __global__ void __launch_bounds__(C::THREADS)
   auto empty_bar = [&](int s) { return bars + 8u * (C::STAGES + s); };
   const u32 done_bar = bars + 8u * (2 * C::STAGES);
   u32 *tmem_slot = reinterpret_cast<u32 *>(smem + C::BAR_OFF + C::NBARS * 8);
+  volatile u32 *failed = tmem_slot + 1;
   u32 *status = g.epi.status;
   int *tab_off = reinterpret_cast<int *>(smem + C::TAB_OFF);
   int *tab_tile = tab_off + kMaxGroups + 1;
@@ -1368,6 +1376,7 @@ __global__ void __launch_bounds__(C::THREADS)
       mbar_init(empty_bar(s), 1);
     }
     mbar_init(done_bar, 1);
+    *failed = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tmap_w);
     tma_prefetch_desc(&tmap_x);
@@ -1409,6 +1418,11 @@ __global__ void __launch_bounds__(C::THREADS)
   const int kb0 = static_cast<int>(static_cast<long long>(nkb) * rank / S);
   const int kb1 = static_cast<int>(static_cast<long long>(nkb) * (rank + 1) / S);
   const int rows = min(C::BN, row_end - m0);
+
+  // one thread, before the cluster meets
+  auto fail = [&] {
+    for (int c = 0; c < S; ++c) st_cluster_u32(mapa_cluster(smem_u32(tmem_slot + 1), c), 1);
+  };
 
   auto load_w = [&](int s, int kb) {
     const u32 sw = base + s * C::STAGE_BYTES;
@@ -1467,10 +1481,16 @@ __global__ void __launch_bounds__(C::THREADS)
       }
     } else if (warp == 1) {
       if (elect_one()) {
+        // X comes behind the previous kernel, which may take any time: the
+        // bounded wait begins only when that has ended
+        if (!g.wait_last) pdl_wait();
         int s = 0;
         u32 ph = 0;
         for (int kb = kb0; kb < kb1; ++kb) {
-          if (!mbar_wait(full_bar(s), ph, status, 0x52)) break;
+          if (!mbar_wait(full_bar(s), ph, status, 0x52)) {
+            fail();
+            break;
+          }
           tc_fence_after();
           const u32 sw = base + s * C::STAGE_BYTES, sx = sw + C::W_BYTES;
 #pragma unroll
@@ -1497,7 +1517,10 @@ __global__ void __launch_bounds__(C::THREADS)
       if (!g.wait_last) pdl_wait();  // bias, residual and outputs are ordered after the previous kernel
       const int q = warp & 3;
       bool ok = true;
-      if (lane == 0) ok = mbar_wait(done_bar, 0, status, 0x53);
+      if (lane == 0) {
+        ok = mbar_wait(done_bar, 0, status, 0x53);
+        if (!ok) fail();
+      }
       ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
       tc_fence_after();
       if (ok) {
@@ -1526,7 +1549,7 @@ __global__ void __launch_bounds__(C::THREADS)
     else
       __syncthreads();
 
-    if (warp >= 2) {
+    if (warp >= 2 && !*failed) {
       const Epilogue &p = g.epi;
       const int col = n0 + 4 * lane;
       const float alpha = p.group_scale ? p.alpha * __ldcg(p.group_scale + grp) : p.alpha;
