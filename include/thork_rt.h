@@ -330,8 +330,11 @@ THORK_API int thork_skinny_gemm_bf16_noalloc_status(unsigned *status, int clear,
  * (the status word is allocated by the first call on a device, and a kernel
  * is loaded by its first, so make one call of the same sizes before a stream
  * capture).  Arrays are dense row-major device memory,
- * 16-byte aligned; bf16 unless said otherwise; sizes are at most 2^30.  Sums
- * are fp32; every output is rounded once.                                  */
+ * 16-byte aligned; bf16 unless said otherwise.  Sizes are at most 2^30, and
+ * those that a product sums over (K; for gradients N of dA, and M or T of dB)
+ * at most 2^23.  Sums are fp32, by tensor cores, which cut each product to the
+ * running sum's last bits (2^-25 of it: of 2^23 equal terms in one tile 1.4 %
+ * was lost); every output is rounded once.                                 */
 enum {
   THORK_ACT_NONE = 0,
   THORK_ACT_RELU = 1,

@@ -55,3 +55,44 @@ def test_a_product_behind_a_slow_kernel_waits_for_it(m, n, k):
     assert rt.kernel_status() == 0
     z, err = product(wide(a), wide(b))
     close(out.to_host(), act(z, "silu"), act_err(z, err), "out")
+
+
+def _threes(*shape):
+    d = rt.empty(shape, np.uint16)
+    rt.check(rt.lib().thork_memset(d.ptr, 0x40, d.nbytes, None))  # 0x4040: 3.0
+    return d
+
+
+LONGEST = 1 << 23
+
+
+def _all_of_it(out):
+    """2^23 products of 9, summed by tensor cores, which may cut a product to
+    the running sum's last bit (74.5e6 measured without a split, 75.5e6 with
+    one).  The sum stays below 2^27, so that bit is at most 8, and of each 9 at
+    least 8 is added; 2^26 and 9 2^23 are bf16 numbers."""
+    got = wide(out.to_host())
+    assert ((got >= 8.0 * LONGEST) & (got <= 9.0 * LONGEST)).all(), got
+
+
+@pytest.mark.parametrize("rows", [2, 32])
+def test_the_longest_contraction_of_a_product(rows):
+    """One tile, whose accumulator is waited for through 131072 blocks
+    (swap_kernel splits them; rows_kernel, which 32 rows a group go to, does
+    not)."""
+    a, b = _threes(rows, LONGEST), _threes(1, LONGEST, 8)
+    out = rt.empty((rows, 8), np.uint16)
+    out.zero()
+    tk.kernels.grouped_matmul(1, rows, 8, LONGEST)(out, a, b, np.array([0, rows], np.int32))
+    _all_of_it(out)
+
+
+def test_the_longest_contraction_of_a_gradient():
+    a, dout = _threes(LONGEST, 8), _threes(LONGEST, 8)
+    db = rt.empty((1, 8, 8), np.uint16)
+    for call in (lambda: tk.kernels.grouped_matmul_backward(1, LONGEST, 8, 8)(
+                     None, db, dout, a, None, np.array([0, LONGEST], np.int32)),
+                 lambda: tk.kernels.linear_backward(LONGEST, 8, 8)(None, db, None, dout, a, None)):
+        db.zero()
+        call()
+        _all_of_it(db)

@@ -344,6 +344,18 @@ int check_sizes(int rows, int n, int k, int align, const char *what) {
   return THORK_OK;
 }
 
+// An epilogue waits for the whole contraction of its tile, at most
+// THORK_WAIT_TIMEOUT_NS (1 s).  A block of the contraction is 64 values (e4m3:
+// 128) and takes 0.3 us of a tile at the tensor pipe's rate and at most 1.5 us
+// where every CTA's operands come from HBM, so 2^23 values stay below 0.2 s.
+constexpr int kMaxContraction = 1 << 23;
+
+int check_contraction(int len, const char *name, const char *what) {
+  if (len > kMaxContraction)
+    return thork_set_error(THORK_ERR_INVALID, "%s: a contraction over %s=%d is more than 2^23", what, name, len);
+  return THORK_OK;
+}
+
 int check_groups(int groups, const void *offsets, const char *what) {
   if (groups < 1 || groups > kMaxGroups)
     return thork_set_error(THORK_ERR_INVALID, "%s: E=%d must be 1..%d", what, groups, kMaxGroups);
@@ -384,6 +396,7 @@ int linear(const void *a, const void *b, void *c, const void *bias, const void *
            int M, int N, int K, float alpha, int act, int flags, void *stream, const char *what) {
   int rc;
   if ((rc = check_sizes(M, N, K, KIND == KIND_BF16 ? 8 : 16, what))) return rc;
+  if ((rc = check_contraction(K, "K", what))) return rc;
   if ((rc = check_act(act, what))) return rc;
   if (flags & ~THORK_LINEAR_W_STATIC)
     return thork_set_error(THORK_ERR_INVALID, "%s: unknown flags 0x%x", what, flags);
@@ -410,6 +423,7 @@ int grouped(const void *a, const void *b, void *c, const int *offsets, void *pre
             const char *what) {
   int rc;
   if ((rc = check_sizes(T, N, K, KIND == KIND_BF16 ? 8 : 16, what))) return rc;
+  if ((rc = check_contraction(K, "K", what))) return rc;
   if ((rc = check_groups(E, offsets, what))) return rc;
   if ((rc = check_act(act, what))) return rc;
   if (flags & ~THORK_LINEAR_W_STATIC)
@@ -438,6 +452,8 @@ int backward(void *da, void *db, float *dbias, const void *dout, const void *a, 
              int act, void *stream, const char *what) {
   int rc;
   if ((rc = check_sizes(rows, N, K, 8, what))) return rc;
+  if (da && (rc = check_contraction(N, "N", what))) return rc;
+  if (db && (rc = check_contraction(rows, groups ? "T" : "M", what))) return rc;
   if ((rc = check_act(act, what))) return rc;
   const bool bent = act != THORK_ACT_NONE;
   if (bent != (preact != nullptr) || bent != (dpre != nullptr))

@@ -11,7 +11,7 @@ to the host and a call can be captured into a graph that later sizes reuse.
 from .. import dtypes as dt
 from .. import runtime as rt
 from ._library import Operand, run_operands
-from .linear import activation_code, check_preact, check_sizes
+from .linear import MAX_CONTRACTION, activation_code, check_contraction, check_preact, check_sizes
 
 MAX_GROUPS = 1024
 
@@ -37,7 +37,8 @@ class grouped_matmul:
     With ``dtype=tk.dt.float8_e4m3`` the call takes ``scale_a`` (a number) and
     ``scale_b`` (float32 ``[E]``, one per expert, or ``None`` for ones):
     ``z[r] = scale_a * scale_b[e] * (A[r] @ B[e])``.  ``activation``,
-    ``preact`` and ``static_weights`` are as for ``tk.kernels.linear``.
+    ``preact`` and ``static_weights`` are as for ``tk.kernels.linear``.  K is
+    at most 2^23.
     """
 
     name = "grouped_matmul"
@@ -46,6 +47,7 @@ class grouped_matmul:
                  activation: str = "none", static_weights: bool = False):
         E, T, N, K = int(E), int(T), int(N), int(K)
         _check("grouped_matmul", dtype, E, T, N, K)
+        check_contraction("grouped_matmul", "K", K)
         self._fp8 = dtype == dt.float8_e4m3
         self._sizes = (E, T, N, K)
         self._act = (activation_code(activation, "grouped_matmul"), int(bool(static_weights)))
@@ -82,7 +84,7 @@ class grouped_matmul_backward:
     ``dB[E, K, N]`` is written whole (zeros for an empty expert); rows outside
     every group are left as they were in ``dA`` and ``dpre``.  ``dA`` or ``dB``
     may be ``None``; ``preact`` and ``dpre`` are as for
-    ``tk.kernels.linear_backward``.
+    ``tk.kernels.linear_backward``.  N is at most 2^23 for ``dA``, T for ``dB``.
     """
 
     name = "grouped_matmul_backward"
@@ -108,6 +110,11 @@ class grouped_matmul_backward:
         check_preact(self.name, self._bent, preact, dpre)
         if dout is None or offsets is None or (dB is not None and A is None) or (dA is not None and B is None):
             raise TypeError("grouped_matmul_backward: dout and offsets are required, A for dB and B for dA")
+        T, N = self._tail[1:3]
+        if T > MAX_CONTRACTION and dB is not None:
+            check_contraction(self.name, "T", T)
+        if N > MAX_CONTRACTION and dA is not None:
+            check_contraction(self.name, "N", N)
         fn = rt.lib().thork_grouped_gemm_backward_bf16
         run_operands(self._operands, (dA, dB, dout, A, B, offsets, preact, dpre),
                      lambda p, s: fn(*p, *self._tail, s), self.name, stream, sync)

@@ -22,6 +22,16 @@ def activation_code(activation: str, what: str) -> int:
     return ACTIVATIONS[activation]
 
 
+# what a product may sum over: an epilogue's bounded wait spans its tile's whole
+# contraction (csrc/linear.cu, kMaxContraction)
+MAX_CONTRACTION = 1 << 23
+
+
+def check_contraction(what: str, name: str, size: int) -> None:
+    if size > MAX_CONTRACTION:
+        raise ValueError(f"{what}: a contraction over {name}={size} is more than 2^23")
+
+
 def check_sizes(what: str, dtype: dt.Dtype, N: int, K: int, **positive) -> None:
     for name, v in {**positive, "N": N, "K": K}.items():
         if not 0 < v <= 1 << 30:
@@ -43,7 +53,8 @@ class linear:
     bf16 for ``linear_backward``.  ``out`` may be the residual itself.  With
     ``dtype=tk.dt.float8_e4m3`` the call takes ``scale_a`` and ``scale_b`` and
     ``z = scale_a * scale_b * (A @ B) + bias``; everything but A and B stays
-    bf16.  K and N are multiples of 8 (e4m3: 16), M is any.
+    bf16.  K and N are multiples of 8 (e4m3: 16), M is any positive number; K
+    is at most 2^23.
 
     ``static_weights``: B is written by no earlier kernel on the stream
     (decode weights), so that a product of few rows may start fetching it
@@ -56,6 +67,7 @@ class linear:
                  activation: str = "none", static_weights: bool = False):
         M, N, K = int(M), int(N), int(K)
         check_sizes("linear", dtype, N, K, M=M)
+        check_contraction("linear", "K", K)
         act, flags = activation_code(activation, "linear"), int(bool(static_weights))
         self._fp8 = dtype == dt.float8_e4m3
         self._operands = (
@@ -95,7 +107,8 @@ class linear_backward:
     the call needs ``preact`` as the forward pass left it and ``dpre``, an
     [M, N] output that the two products read; without one ``dpre`` is ``dout``
     and both stay ``None``.  ``dbias`` is float32 (its sum is taken before
-    ``dpre`` is rounded), the other outputs are bf16.
+    ``dpre`` is rounded), the other outputs are bf16.  N is at most 2^23 for
+    ``dA``, M for ``dB``.
     """
 
     name = "linear_backward"
@@ -119,6 +132,11 @@ class linear_backward:
         check_preact(self.name, self._bent, preact, dpre)
         if dout is None or (dB is not None and A is None) or (dA is not None and B is None):
             raise TypeError("linear_backward: dout is required, A for dB and B for dA")
+        M, N = self._tail[:2]
+        if M > MAX_CONTRACTION and dB is not None:
+            check_contraction(self.name, "M", M)
+        if N > MAX_CONTRACTION and dA is not None:
+            check_contraction(self.name, "N", N)
         fn = rt.lib().thork_linear_backward_bf16
         run_operands(self._operands, (dA, dB, dbias, dout, A, B, preact, dpre),
                      lambda p, s: fn(*p, *self._tail, s), self.name, stream, sync)
