@@ -96,3 +96,27 @@ def test_the_longest_contraction_of_a_gradient():
         db.zero()
         call()
         _all_of_it(db)
+
+
+def test_a_status_that_says_a_wait_expired_is_raised():
+    """A status planted in the device's word, as a kernel leaves it whose wait
+    expired: asynchronous calls leave it there, the next call that
+    synchronises raises it and clears it; its own output is as ever."""
+    m, n, k = 5, 264, 136
+    rng = np.random.default_rng(2)
+    a, b = bits(rng, m, k), bits(rng, k, n, std=0.1)
+    want, out = np.zeros((m, n), np.uint16), np.zeros((m, n), np.uint16)
+    f = tk.kernels.linear(m, n, k)
+    f(want, a, b)
+    A, B, O = rt.to_device(a), rt.to_device(b), rt.empty((m, n), np.uint16)
+    s = rt.Stream()
+    word = np.array([1 | 0x53 << 8], np.uint32)
+    for call in (lambda: f(O, A, B, stream=s), lambda: f(out, a, b, stream=s, sync=False)):
+        rt.copy_htod(rt.status_pointer(), word)
+        f(O, A, B, stream=s, sync=False)
+        with pytest.raises(rt.CudaError, match="bounded wait expired at site 83"):
+            call()
+        assert rt.kernel_status() == 0
+        np.testing.assert_array_equal(O.to_host(), want)
+    f(out, a, b)
+    np.testing.assert_array_equal(out, want)

@@ -51,3 +51,88 @@ def test_c_entry_points_refuse_long_contractions_and_only_those():
     bad(L.thork_linear_bf16(16, 32, 48, None, None, None, LONG, 64, 64, 7, 0, None), "activation")
     bad(bwd(16, None, None, 64, None, 96, None, None, LONG, 64, 64, 7, None), "activation")
     bad(bwd(None, 32, None, 64, 80, None, None, None, 4, LONG, 64, 7, None), "activation")
+
+
+# ---------------------------------------------------------------- the host side of a call
+class _Fake:
+    """The runtime under a call, without a device: a stream, buffers and
+    copies that record what happens in order."""
+
+    def __init__(self, monkeypatch, status=0):
+        self.log, self.status, self.allocated = [], status, 0
+        fake = self
+
+        class Buffer:
+            def __init__(self, nbytes):
+                fake.allocated += 1
+                self.ptr, self.nbytes, self._dev = 4096 * fake.allocated, nbytes, 0
+
+            def free(self):
+                fake.log.append("free")
+                self.ptr = 0
+
+        class Stream:
+            handle = 4096
+
+            def synchronize(self):
+                fake.log.append("synchronize")
+
+        def read(ref, *_):
+            ref._obj.value = fake.status
+            return 0
+
+        def stream_status(ref, handle):
+            fake.log.append("synchronize")
+            return read(ref)
+
+        def kernel_status(ref, clear):
+            read(ref)
+            if clear:
+                fake.status = 0
+            return 0
+
+        self.Buffer, self.stream = Buffer, Stream()
+        monkeypatch.setattr(rt, "get_device", lambda: 0)
+        monkeypatch.setattr(rt, "DeviceBuffer", Buffer)
+        monkeypatch.setattr(rt, "copy_htod", lambda *a, **k: self.log.append("in"))
+        monkeypatch.setattr(rt, "copy_dtoh", lambda *a, **k: self.log.append("out"))
+        for name, f in (("thork_stream_status", stream_status), ("thork_kernel_status", kernel_status)):
+            monkeypatch.setattr(rt.lib(), name, f, raising=False)
+
+    def kernel(self, monkeypatch, name, rc=0):
+        def launch(*args):
+            self.log.append("launch")
+            return rc
+        monkeypatch.setattr(rt.lib(), name, launch, raising=False)
+
+    def array(self, *shape):
+        d = rt.DeviceArray(shape, np.uint16, buffer=self.Buffer(2 * int(np.prod(shape))))
+        return d
+
+
+def test_an_expired_wait_is_raised_by_calls_that_synchronise(monkeypatch):
+    expired = 1 | 0x53 << 8
+    fake = _Fake(monkeypatch, expired)
+    fake.kernel(monkeypatch, "thork_linear_bf16")
+    f = K.linear(4, 64, 64)
+    out, a, b = fake.array(4, 64), fake.array(4, 64), fake.array(64, 64)
+    f(out, a, b, stream=fake.stream, sync=False)  # an asynchronous call reads nothing
+    assert fake.log == ["launch"] and fake.status == expired
+    with pytest.raises(rt.CudaError, match="bounded wait expired at site 83") as e:
+        f(out, a, b, stream=fake.stream)
+    assert e.value.code == rt.ERR_KERNEL and fake.status == 0  # raised once
+    f(out, a, b, stream=fake.stream)
+    # host arrays: the call synchronises in any case
+    fake.status = expired
+    host = np.zeros((4, 64), np.uint16)
+    with pytest.raises(rt.CudaError, match="bounded wait"):
+        f(host, a, b, stream=fake.stream, sync=False)
+
+
+def test_wrong_offsets_stay_in_the_status_word(monkeypatch):
+    bad_offsets = 2 | 0x40 << 8
+    fake = _Fake(monkeypatch, bad_offsets)
+    fake.kernel(monkeypatch, "thork_grouped_gemm_bf16")
+    x, w = np.zeros((4, 64), np.uint16), np.zeros((2, 64, 64), np.uint16)
+    K.grouped_matmul(2, 4, 64, 64)(x.copy(), x, w, np.array([0, 9, 4], np.int32), stream=fake.stream)
+    assert fake.status == bad_offsets

@@ -93,6 +93,19 @@ extern "C" int thork_kernel_status(unsigned *status, int clear) {
   return THORK_OK;
 }
 
+extern "C" int thork_stream_status(unsigned *status, void *stream) {
+  if (!status) return thork_set_error(THORK_ERR_INVALID, "status is NULL");
+  unsigned *d;
+  int rc = thork_status_word(&d);
+  if (rc) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e = cudaMemcpyAsync(status, d, sizeof(unsigned), cudaMemcpyDeviceToHost, s);
+  if (e != cudaSuccess) return thork_cuda_error(e, "read status word");
+  e = cudaStreamSynchronize(s);
+  if (e != cudaSuccess) return thork_cuda_error(e, "cudaStreamSynchronize");
+  return THORK_OK;
+}
+
 extern "C" int thork_status_pointer(void **d_status) {
   if (!d_status) return thork_set_error(THORK_ERR_INVALID, "d_status is NULL");
   unsigned *d;

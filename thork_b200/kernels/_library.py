@@ -127,7 +127,8 @@ def run_operands(operands: Sequence[Operand], args: Sequence, launch: Callable, 
                  stream: Optional["rt.Stream"] = None, sync: bool = True) -> None:
     """Like ``run`` for operands that may be ``None``: checks ``args``, calls
     ``launch(pointers, stream_handle)`` with ``None`` for those left out, and
-    copies host arrays in and written ones back."""
+    copies host arrays in and written ones back.  A call that synchronises
+    (``sync``, or host arrays) raises when a bounded wait has expired."""
     dev = rt.get_device()
     s = stream if stream is not None else rt._dispatch_stream()
     DeviceArray = rt.DeviceArray
@@ -164,9 +165,8 @@ def run_operands(operands: Sequence[Operand], args: Sequence, launch: Callable, 
         if owned is not None:
             for a, ptr in back:
                 rt.copy_dtoh(a, ptr, s, sync=False)
-            s.synchronize()
-        elif sync:
-            s.synchronize()
+        if sync or owned is not None:
+            rt.finish_stream(s, what)
     finally:
         if owned is not None:
             for b in owned:

@@ -87,6 +87,7 @@ _SIGNATURES = {
     "thork_launch": [_vp, ctypes.POINTER(_u), ctypes.POINTER(_u), ctypes.POINTER(_u), _u, _vp, _pvp],
     "thork_tensor_map_2d": [_vp, _i, _vp, _u64, _u64, _u64, _u32, _u32, _i],
     "thork_kernel_status": [ctypes.POINTER(_u), _i],
+    "thork_stream_status": [ctypes.POINTER(_u), _vp],
     "thork_status_pointer": [_pvp],
     "thork_matrix_add_f32": [_vp, _vp, _vp, _sz, _vp],
     "thork_gemm_bf16": [_vp, _vp, _vp, _i, _i, _i, _i, _vp],
@@ -242,6 +243,15 @@ def check_kernel_status(what: str) -> None:
         raise CudaError(
             f"kernel {what} reported status 0x{st:x} (a bounded wait expired at site "
             f"{(st >> 8) & 0xFF})", ERR_KERNEL)
+
+
+def finish_stream(stream: "Stream", what: str) -> None:
+    """Wait for ``stream`` and raise if a bounded wait has expired, in this
+    call's kernels or in ones queued earlier whose status nobody has read."""
+    v = ctypes.c_uint(0)
+    check(lib().thork_stream_status(ctypes.byref(v), stream.handle), what)
+    if v.value & 1:
+        check_kernel_status(what)
 
 
 # --------------------------------------------------------------------------
