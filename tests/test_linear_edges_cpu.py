@@ -136,3 +136,18 @@ def test_wrong_offsets_stay_in_the_status_word(monkeypatch):
     x, w = np.zeros((4, 64), np.uint16), np.zeros((2, 64, 64), np.uint16)
     K.grouped_matmul(2, 4, 64, 64)(x.copy(), x, w, np.array([0, 9, 4], np.int32), stream=fake.stream)
     assert fake.status == bad_offsets
+
+
+def test_a_gathered_result_is_an_operand(monkeypatch):
+    """The arrays that a fused gather returns borrow its slots; they feed a
+    linear layer like any other array of the device."""
+    from thork_b200.dist import _View
+    fake = _Fake(monkeypatch)
+    fake.kernel(monkeypatch, "thork_linear_bf16")
+    gathered = rt.DeviceArray((4, 64), np.uint16, buffer=_View(1 << 20, 512))
+    f = K.linear(4, 64, 64)
+    f(fake.array(4, 64), gathered, fake.array(64, 64), stream=fake.stream)
+    assert fake.log == ["launch", "synchronize"]
+    f._operands[1].check(gathered, 0)
+    with pytest.raises(ValueError, match="device 0"):
+        f._operands[1].check(gathered, 1)

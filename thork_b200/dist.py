@@ -257,13 +257,13 @@ def multicast_supported() -> bool:
 
 
 class _View:
-    """A borrowed device pointer in the shape ``DeviceArray`` expects of its
-    buffer (no ownership)."""
+    """A borrowed pointer of the current device in the shape ``DeviceArray``
+    expects of its buffer (no ownership)."""
 
-    __slots__ = ("ptr", "nbytes")
+    __slots__ = ("ptr", "nbytes", "_dev")
 
     def __init__(self, ptr: int, nbytes: int):
-        self.ptr, self.nbytes = int(ptr), int(nbytes)
+        self.ptr, self.nbytes, self._dev = int(ptr), int(nbytes), rt.get_device()
 
 
 class FusedGather:
