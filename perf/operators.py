@@ -12,6 +12,7 @@ per expert for the experts' weights.
 """
 
 import math
+import operator
 
 import torch
 
@@ -323,9 +324,13 @@ def _plain_grouped_backward(s):
 # ---------------------------------------------------------------------------
 # the framework's calls
 # ---------------------------------------------------------------------------
+# what of a state is wrapped for the framework's call
+_BUFFERS = ("A", "B", "b", "res", "out", "pre", "offsets", "scale_b", "dout", "z", "dz", "dA", "dB", "db")
+
+
 def _own_call(s):
     """The operator's handle and the arguments that a program keeps for it:
-    device arrays over the state's buffers, and the stream they are used on."""
+    device arrays over the state's buffers."""
     import numpy as np
 
     import thork_b200 as tk
@@ -339,7 +344,6 @@ def _own_call(s):
                  torch.float32: np.float32, torch.int32: np.int32}[t.dtype]
         return rt.wrap_pointer(t.data_ptr(), tuple(t.shape), as_np, owner=t)
 
-    stream = rt.Stream.from_handle(torch.cuda.current_stream().cuda_stream)
     act = s["act"]
     dtype = tk.dt.float8_e4m3 if s.get("dtype") == "e4m3" else tk.dt.bfloat16
     a, b = arr(s["A"]), arr(s["B"])
@@ -378,16 +382,31 @@ def _own_call(s):
         got = {"dA": s["dA"], "dB": s["dB"]}
         if act != "none":
             got["dz"] = s["dz"]
-    return f, args, kw, stream, got
+    return f, args, kw, got
+
+
+def _own(s):
+    """The framework's call on torch's current stream; the wraps are made anew
+    for a state whose buffers are others than at the call before."""
+    kept = s.get("call")
+    if kept is None or any(map(operator.is_not, kept["pick"](s), kept["buffers"])):
+        pick = operator.itemgetter(*(name for name in _BUFFERS if s.get(name) is not None))
+        kept = s["call"] = {"pick": pick, "buffers": pick(s), "call": _own_call(s), "handle": -1}
+    # torch.cuda.current_stream().cuda_stream without the Stream object, which
+    # takes longer to make than the rest of this function
+    handle = torch._C._cuda_getCurrentRawStream(kept["buffers"][0].device.index)
+    if handle != kept["handle"]:
+        from thork_b200 import runtime
+
+        kept["handle"], kept["stream"] = handle, runtime.Stream.from_handle(handle)
+    f, args, kw, got = kept["call"]
+    f(*args, **kw, stream=kept["stream"], sync=False)
+    return got
 
 
 def run(state):
     if own:
-        if "call" not in state:
-            state["call"] = _own_call(state)
-        f, args, kw, stream, got = state["call"]
-        f(*args, **kw, stream=stream, sync=False)
-        return got
+        return _own(state)
     return {"linear": _plain_linear, "linear_backward": _plain_linear_backward,
             "grouped": _plain_grouped, "grouped_backward": _plain_grouped_backward}[state["op"]](state)
 
