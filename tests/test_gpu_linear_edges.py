@@ -120,3 +120,48 @@ def test_a_status_that_says_a_wait_expired_is_raised():
         np.testing.assert_array_equal(O.to_host(), want)
     f(out, a, b)
     np.testing.assert_array_equal(out, want)
+
+
+@pytest.mark.parametrize("which", ["linear ragged 777", "linear backward 200", "grouped backward odd"])
+def test_measured_calls_follow_the_current_stream(which):
+    """The calls of perf/operators.py on one state: eager, on another stream,
+    captured and replayed, with a buffer replaced."""
+    import importlib.util
+    import os
+
+    torch = pytest.importorskip("torch")
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "perf", "operators.py")
+    spec = importlib.util.spec_from_file_location("measured_operators", path)
+    ops = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ops)
+    ops.own = True
+    case = next(c for c in ops.listed() if c["name"] == which)
+    state = ops.prepare(case, 3)
+    before = {name: x.clone() for name, x in ops.run(state).items()}
+
+    def fresh():
+        for x in ops.run(state).values():  # rows behind the last group keep their values
+            if "e" not in case:
+                x.zero_()
+
+    fresh()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = ops.run(state)
+    side.synchronize()  # the call's own stream: its results are there
+    for name, x in got.items():
+        assert torch.equal(x, before[name]), name
+    fresh()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = ops.run(state)
+    graph.replay()
+    torch.cuda.synchronize()
+    for name, x in got.items():
+        assert torch.equal(x, before[name]), name
+    state["A"] = state["A"].clone()
+    for name, x in ops.run(state).items():
+        assert torch.equal(x, before[name]), name
+    assert state["call"]["buffers"][0] is state["A"]
