@@ -151,3 +151,37 @@ def test_a_gathered_result_is_an_operand(monkeypatch):
     f._operands[1].check(gathered, 0)
     with pytest.raises(ValueError, match="device 0"):
         f._operands[1].check(gathered, 1)
+
+
+def _call_linear(fake, **kw):
+    host = [np.zeros(s, np.uint8) for s in ((4, 64), (64, 64))]
+    K.linear(4, 64, 64, tk.dt.float8_e4m3)(np.zeros((4, 64), np.uint16), *host, stream=fake.stream, **kw)
+
+
+def test_a_call_that_fails_waits_for_its_copies_before_it_frees(monkeypatch):
+    """Copies of host arrays are queued before the launch is refused: their
+    buffers go back to the pool only when the stream has finished."""
+    fake = _Fake(monkeypatch)
+    fake.kernel(monkeypatch, "thork_linear_e4m3", rc=rt.ERR_INVALID)
+    with pytest.raises(rt.CudaError):
+        _call_linear(fake)
+    assert fake.log == ["in", "in", "launch", "synchronize", "free", "free", "free"]
+
+    fake.log.clear()
+
+    def raises(*args):
+        raise TypeError("scale_a")
+
+    monkeypatch.setattr(rt.lib(), "thork_linear_e4m3", raises, raising=False)
+    with pytest.raises(TypeError):
+        _call_linear(fake, scale_a="one")
+    assert fake.log == ["in", "in", "synchronize", "free", "free", "free"]
+
+
+def test_an_operand_refused_after_others_were_copied_waits_too(monkeypatch):
+    fake = _Fake(monkeypatch)
+    fake.kernel(monkeypatch, "thork_linear_bf16")
+    x, w = np.zeros((4, 64), np.uint16), np.zeros((64, 63), np.uint16)
+    with pytest.raises(ValueError):
+        K.linear(4, 64, 64)(x.copy(), x, w, stream=fake.stream)
+    assert fake.log == ["in", "synchronize", "free", "free"]

@@ -167,6 +167,10 @@ def run_operands(operands: Sequence[Operand], args: Sequence, launch: Callable, 
                 rt.copy_dtoh(a, ptr, s, sync=False)
         if sync or owned is not None:
             rt.finish_stream(s, what)
+    except BaseException:
+        if owned:
+            s.synchronize()  # copies into the buffers may be in flight
+        raise
     finally:
         if owned is not None:
             for b in owned:
