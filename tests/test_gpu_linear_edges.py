@@ -3,12 +3,14 @@ before them, status words, extreme values (tolerances derived in
 linear_ref.py)."""
 
 import ctypes
+import math
 
 import numpy as np
 import pytest
 
 import thork_b200 as tk
-from linear_ref import act, act_err, bits, close, product, wide
+from linear_ref import BF16, act, act_err, bits, close, product, wide
+from oracle import oracle
 
 pytestmark = pytest.mark.gpu
 rt = tk.runtime
@@ -165,3 +167,86 @@ def test_measured_calls_follow_the_current_stream(which):
     for name, x in ops.run(state).items():
         assert torch.equal(x, before[name]), name
     assert state["call"]["buffers"][0] is state["A"]
+
+
+# ---------------------------------------------------------------- activations on a grid
+# Relative error of an activation beside the output's rounding: the exponent of
+# its exponential is a product of three factors, up to 126, rounded twice or
+# three times (3 2^-24 126 ln 2 = 1.6e-5 of the value); Phi's tail adds its
+# approximation's 5e-5; exponential, reciprocal and the rest add a few 2^-22.
+# Together below 2^-13.  Exponentials and sigmoids below 2^-126 may be 0.
+ACT_REL = 2.0 ** -13
+TINY = 2.0 ** -125
+_erfc = np.vectorize(math.erfc, otypes=[np.float64])
+
+
+def _grid(last):
+    """Every bf16 value of magnitude 2^-20 to `last`, both signs."""
+    top = int(oracle.f32_to_bf16_bits(np.array([last], np.float32))[0])
+    up = np.arange(0x3580, top + 1, dtype=np.uint16)
+    return np.concatenate([up, up | 0x8000])
+
+
+def _gate(z, activation):
+    """(gate, its derivative) of an activation z * gate(z), without cancellation."""
+    if activation == "gelu":
+        return 0.5 * _erfc(-z / math.sqrt(2)), np.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    u, du = z, 1.0
+    if activation == "gelu_tanh":
+        c = 2 * math.sqrt(2 / math.pi)
+        u, du = c * (z + 0.044715 * z ** 3), c * (1 + 3 * 0.044715 * z * z)
+    e = np.exp(-np.abs(u))
+    return np.where(u > 0, 1, e) / (1 + e), du * e / (1 + e) ** 2
+
+
+@pytest.mark.parametrize("rows", [24, 4096])
+@pytest.mark.parametrize("activation,last", [("gelu", 14.0), ("gelu_tanh", 9.0), ("silu", 100.0)])
+def test_activations_are_relatively_accurate(activation, last, rows):
+    """z = A B with one non-zero product, exact; z * gate(z) keeps its relative
+    accuracy down the negative tail, where it is far below one."""
+    bits_z = _grid(last)
+    a = np.zeros((rows, 8), np.uint16)
+    b = np.full((8, 256), 0x3F80, np.uint16)  # 1
+    f = tk.kernels.linear(rows, 256, 8, activation=activation)
+    for first in range(0, len(bits_z), rows):
+        part = bits_z[first:first + rows]
+        if rows < 100 and first // rows % 8:
+            continue  # few rows go to another kernel; an eighth of the grid does
+        a[:len(part), 0] = part
+        out, pre = np.zeros((rows, 256), np.uint16), np.zeros((rows, 256), np.uint16)
+        f(out, a, b, preact=pre)
+        out, pre = out[:len(part)], pre[:len(part)]
+        np.testing.assert_array_equal(pre, np.repeat(part[:, None], 256, 1))
+        z = wide(part)
+        gate, _ = _gate(z, activation)
+        want = z * gate
+        tol = (BF16 + ACT_REL) * np.abs(want) + TINY * np.abs(z)
+        off = np.abs(wide(out) - want[:, None])
+        worst = np.argmax(off.max(1) - tol)
+        assert (off <= tol[:, None]).all(), f"z = {z[worst]}: {wide(out)[worst].max()}, not {want[worst]}"
+
+
+@pytest.mark.parametrize("activation,last", [("gelu", 14.0), ("gelu_tanh", 9.0), ("silu", 100.0)])
+def test_slopes_are_relatively_accurate(activation, last):
+    """gate + z gate', each term to ACT_REL of itself (the sum passes zero).
+    Where the gate is close to 1, 1 - gate is off by a rounding of 2^-24, which
+    z and the inner derivative (at most 3 |z| + 3 for these z) multiply."""
+    bits_z = _grid(last)
+    m, n = 64, 256
+    for first in range(0, len(bits_z), m * n):
+        part = bits_z[first:first + m * n]
+        pre = np.zeros(m * n, np.uint16)
+        pre[:len(part)] = part
+        dout = np.full((m, n), 0x3F80, np.uint16)
+        dpre = np.zeros((m, n), np.uint16)
+        tk.kernels.linear_backward(m, n, 8, activation=activation)(
+            None, None, None, dout, None, None, pre.reshape(m, n), dpre)
+        z = wide(part)
+        gate, slope = _gate(z, activation)
+        want = gate + z * slope
+        got = wide(dpre).reshape(-1)[:len(part)]
+        terms = gate + np.abs(z * slope)
+        near_one = 0.0 if activation == "gelu" else 2.0 ** -23 * np.abs(z) * (3 * np.abs(z) + 3) * (gate > 0.5)
+        tol = BF16 * np.abs(want) + 1.01 * (ACT_REL * terms + near_one + TINY * (3 * np.abs(z) + 3) ** 2)
+        worst = np.argmax(np.abs(got - want) - tol)
+        assert (np.abs(got - want) <= tol).all(), f"z = {z[worst]}: {got[worst]}, not {want[worst]} +- {tol[worst]}"
