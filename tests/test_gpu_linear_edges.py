@@ -250,3 +250,22 @@ def test_slopes_are_relatively_accurate(activation, last):
         tol = BF16 * np.abs(want) + 1.01 * (ACT_REL * terms + near_one + TINY * (3 * np.abs(z) + 3) ** 2)
         worst = np.argmax(np.abs(got - want) - tol)
         assert (np.abs(got - want) <= tol).all(), f"z = {z[worst]}: {got[worst]}, not {want[worst]} +- {tol[worst]}"
+
+
+@pytest.mark.parametrize("activation", ["relu", "gelu", "gelu_tanh", "silu"])
+def test_the_largest_values(activation):
+    """From 2^8 to bf16's largest number an activation is z or 0 and its slope
+    1 or 0 (the next terms are below e^-200): nothing overflows on the way."""
+    up = np.arange(0x4380, 0x7F80, dtype=np.uint16)
+    part = np.concatenate([up, up | 0x8000])
+    z = wide(part)
+    rows = len(part)
+    a = np.zeros((rows, 8), np.uint16)
+    a[:, 0] = part
+    out = np.zeros((rows, 8), np.uint16)
+    tk.kernels.linear(rows, 8, 8, activation=activation)(out, a, np.full((8, 8), 0x3F80, np.uint16))
+    np.testing.assert_array_equal(wide(out), np.repeat(np.maximum(z, 0)[:, None], 8, 1))
+    dout, dpre = np.full((rows, 8), 0x3F80, np.uint16), np.zeros((rows, 8), np.uint16)
+    tk.kernels.linear_backward(rows, 8, 8, activation=activation)(
+        None, None, None, dout, None, None, np.repeat(part[:, None], 8, 1), dpre)
+    np.testing.assert_array_equal(wide(dpre), np.repeat((z > 0)[:, None].astype(np.float64), 8, 1))

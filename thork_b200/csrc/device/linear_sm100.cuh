@@ -257,7 +257,9 @@ __device__ __forceinline__ F2 act_slope(F2 z, int act) {
     const F2 zz = z * z;
     const F2 p = sigmoid_exp2(z * fma2(zz, f2(-kTanh1 * kLog2e), f2(-kTanh0 * kLog2e)));
     const F2 q = fma2(p, p * f2(-1.0f), p);  // p (1 - p)
-    return fma2(z * q, fma2(zz, f2(3.0f * kTanh1), f2(kTanh0)), p);
+    // z q first, which is 0 for large |z|, where z^2 overflows (0 times infinity)
+    const F2 w = z * q;
+    return fma2(w * z * z, f2(3.0f * kTanh1), fma2(w, f2(kTanh0), p));
   }
   const F2 p = sigmoid_exp2(z * f2(-kLog2e));
   const F2 q = fma2(p, p * f2(-1.0f), p);
