@@ -117,6 +117,9 @@ THORK_API int thork_memset(void *d_ptr, int value, size_t nbytes, void *stream);
  * reference counterpart; tests use it to show an entry point allocates
  * nothing.                                                                 */
 THORK_API int thork_mem_info(size_t *free_bytes, size_t *total_bytes);
+/* The device whose memory `ptr` is in: *device is its index, the current one
+ * for managed memory, -1 for host memory and addresses CUDA does not know.  */
+THORK_API int thork_pointer_device(const void *ptr, int *device);
 
 /* ---- streams and events (no reference counterpart: it uses stream 0) --- */
 THORK_API int thork_stream_create(void **stream);

@@ -269,3 +269,18 @@ def test_the_largest_values(activation):
     tk.kernels.linear_backward(rows, 8, 8, activation=activation)(
         None, None, None, dout, None, None, np.repeat(part[:, None], 8, 1), dpre)
     np.testing.assert_array_equal(wide(dpre), np.repeat((z > 0)[:, None].astype(np.float64), 8, 1))
+
+
+def test_host_memory_is_not_wrapped():
+    torch = pytest.importorskip("torch")
+    host, pinned = np.zeros(64, np.uint16), rt.pinned_empty((64,), np.uint16)
+    for x in (host, pinned):
+        with pytest.raises(ValueError, match="not device memory"):
+            rt.wrap_pointer(x.ctypes.data, x.shape, x.dtype)
+    t = torch.arange(64, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    # into the middle of an allocation, and of the framework's own memory
+    np.testing.assert_array_equal(rt.wrap_pointer(t[16:].data_ptr(), (48,), np.int32, owner=t).to_host(),
+                                  np.arange(16, 64))
+    d = rt.to_device(host)
+    assert rt.wrap_pointer(d.ptr, (64,), np.uint16).ptr == d.ptr

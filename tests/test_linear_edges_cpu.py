@@ -185,3 +185,24 @@ def test_an_operand_refused_after_others_were_copied_waits_too(monkeypatch):
     with pytest.raises(ValueError):
         K.linear(4, 64, 64)(x.copy(), x, w, stream=fake.stream)
     assert fake.log == ["in", "synchronize", "free", "free"]
+
+
+def test_only_memory_of_the_current_device_is_wrapped(monkeypatch):
+    where = {4096: 0, 8192: 1, 12288: -1}
+
+    def pointer_device(ptr, ref):
+        ref._obj.value = where[ptr]
+        return 0
+
+    monkeypatch.setattr(rt, "get_device", lambda: 0)
+    monkeypatch.setattr(rt.lib(), "thork_pointer_device", pointer_device, raising=False)
+    owner = object()
+    a = rt.wrap_pointer(4096, (4, 64), np.uint16, owner=owner)
+    assert (a.ptr, a.shape, a.nbytes, a.buffer._dev) == (4096, (4, 64), 512, 0)
+    with pytest.raises(ValueError, match="memory of device 1"):
+        rt.wrap_pointer(8192, (4, 64), np.uint16)
+    with pytest.raises(ValueError, match="not device memory"):
+        rt.wrap_pointer(12288, (4, 64), np.uint16)
+    assert rt.wrap_pointer(0, (0, 64), np.uint16).size == 0
+    monkeypatch.setattr(rt, "get_device", lambda: 1)
+    assert rt.wrap_pointer(8192, (4, 64), np.uint16).buffer._dev == 1

@@ -242,6 +242,15 @@ extern "C" int thork_mem_info(size_t *free_bytes, size_t *total_bytes) {
   CUDA_TRY(cudaMemGetInfo(free_bytes, total_bytes), "cudaMemGetInfo");
   return THORK_OK;
 }
+extern "C" int thork_pointer_device(const void *ptr, int *device) {
+  if (!device) return thork_set_error(THORK_ERR_INVALID, "pointer_device: NULL output");
+  cudaPointerAttributes a = {};
+  CUDA_TRY(cudaPointerGetAttributes(&a, ptr), "cudaPointerGetAttributes");
+  *device = -1;
+  if (a.type == cudaMemoryTypeDevice) *device = a.device;
+  if (a.type == cudaMemoryTypeManaged) CUDA_TRY(cudaGetDevice(device), "cudaGetDevice");
+  return THORK_OK;
+}
 extern "C" int thork_memset(void *d_ptr, int value, size_t n, void *stream) {
   if (n == 0) return THORK_OK;
   CUDA_TRY(cudaMemsetAsync(d_ptr, value, n, static_cast<cudaStream_t>(stream)), "cudaMemsetAsync");

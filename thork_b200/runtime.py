@@ -66,6 +66,7 @@ _SIGNATURES = {
     "thork_memcpy_dtod": [_vp, _vp, _sz, _vp],
     "thork_memset": [_vp, _i, _sz, _vp],
     "thork_mem_info": [ctypes.POINTER(_sz), ctypes.POINTER(_sz)],
+    "thork_pointer_device": [_vp, ctypes.POINTER(_i)],
     "thork_stream_create": [_pvp],
     "thork_stream_destroy": [_vp],
     "thork_stream_synchronize": [_vp],
@@ -462,8 +463,18 @@ class _Borrowed:
 def wrap_pointer(ptr: int, shape, dtype, owner=None) -> DeviceArray:
     """A DeviceArray over C-contiguous device memory of another library, on
     the current device (for example a torch tensor's ``data_ptr()``, with the
-    tensor as ``owner`` so that it outlives the array)."""
+    tensor as ``owner`` so that it outlives the array).  Host memory and
+    memory of another device are refused."""
     dtype = np.dtype(dtype)
+    here = get_device()
+    if ptr:  # an empty tensor's is 0
+        at = ctypes.c_int(-1)
+        check(lib().thork_pointer_device(int(ptr), ctypes.byref(at)), "wrap_pointer")
+        if at.value < 0:
+            raise ValueError(f"wrap_pointer: 0x{int(ptr):x} is not device memory")
+        if at.value != here:
+            raise ValueError(f"wrap_pointer: 0x{int(ptr):x} is memory of device {at.value}; the current "
+                             f"device is {here}")
     return DeviceArray(shape, dtype, buffer=_Borrowed(ptr, math.prod(shape) * dtype.itemsize, owner))
 
 
