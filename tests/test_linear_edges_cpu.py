@@ -206,3 +206,19 @@ def test_only_memory_of_the_current_device_is_wrapped(monkeypatch):
     assert rt.wrap_pointer(0, (0, 64), np.uint16).size == 0
     monkeypatch.setattr(rt, "get_device", lambda: 1)
     assert rt.wrap_pointer(8192, (4, 64), np.uint16).buffer._dev == 1
+
+
+def test_host_outputs_are_writeable_and_apart(monkeypatch):
+    fake = _Fake(monkeypatch)
+    fake.kernel(monkeypatch, "thork_linear_bf16")
+    x, w, out = (np.zeros(s, np.uint16) for s in ((4, 64), (64, 64), (8, 64)))
+    f = K.linear(4, 64, 64)
+    frozen = np.frombuffer(bytes(4 * 64 * 2), np.uint16).reshape(4, 64)
+    with pytest.raises(ValueError, match="'out' is written, but the array is read-only"):
+        f(frozen, x, w, stream=fake.stream)
+    f(out[:4], frozen, w, residual=frozen, stream=fake.stream)  # inputs may be read-only
+    with pytest.raises(ValueError, match="'preact' shares memory with another output"):
+        f(out[:4], x, w, preact=out[:4], stream=fake.stream)
+    with pytest.raises(ValueError, match="'preact' shares memory"):
+        f(out[:4], x, w, preact=out[2:6], stream=fake.stream)
+    f(out[:4], x, w, preact=out[4:], residual=out[:4], stream=fake.stream)  # in place, and a neighbour

@@ -116,6 +116,8 @@ class Operand:
         if host:
             if not a.flags["C_CONTIGUOUS"]:
                 raise ValueError(f"Argument for '{self.name}' must be C-contiguous")
+            if self.written and not a.flags["WRITEABLE"]:
+                raise ValueError(f"Argument for '{self.name}' is written, but the array is read-only")
         elif not a.buffer.ptr:
             raise ValueError(f"Argument for '{self.name}' is an array that has been freed")
         elif a.buffer._dev != dev:
@@ -152,6 +154,8 @@ def run_operands(operands: Sequence[Operand], args: Sequence, launch: Callable, 
                 continue
             if owned is None:
                 owned, back = [], []
+            if o.written and any(np.may_share_memory(a, other) for other, _ in back):
+                raise ValueError(f"{what}: '{o.name}' shares memory with another output")
             buf = rt.DeviceBuffer(a.nbytes)
             owned.append(buf)
             ptrs.append(buf.ptr)
