@@ -396,6 +396,20 @@ THORK_API int thork_grouped_gemm_backward_bf16(void *d_da, void *d_db, const voi
                                                void *d_dpre, int E, int T, int N, int K, int activation,
                                                void *stream);
 
+/* Which kernel a product of these operators takes on a GPU of `sms`
+ * multiprocessors (host arithmetic; needs no GPU): *tile_rows = 0 for the
+ * kernel of many rows, else the rows per tile of the kernel of few rows, whose
+ * contraction is split over *split CTAs.  E is the number of groups (1 without
+ * groups).  dA of a backward pass is the product of N and K exchanged.      */
+enum {
+  THORK_CHOICE_BF16 = 0,          /* out[M,N] over K                        */
+  THORK_CHOICE_E4M3 = 1,
+  THORK_CHOICE_GRADIENT = 2,      /* dB[K,N] over M                         */
+  THORK_CHOICE_GROUPED_BF16 = 3,  /* M is the buffer's rows, T              */
+  THORK_CHOICE_GROUPED_E4M3 = 4
+};
+THORK_API int thork_linear_choice(int form, int M, int N, int K, int E, int sms, int *tile_rows, int *split);
+
 /* ---- NVLink multicast buffers (no reference counterpart) ---------------
  * For the fused GEMM + all-gather over NVSwitch multicast ("NVLS"): every
  * GPU of a group binds memory of its own to one multicast object, and a

@@ -1,9 +1,12 @@
 """CPU: what the linear-layer operators refuse, and what their host side does
 when a call fails."""
 
+import ctypes
+
 import numpy as np
 import pytest
 
+import linear_choices as C
 import thork_b200 as tk
 from thork_b200 import runtime as rt
 
@@ -222,3 +225,39 @@ def test_host_outputs_are_writeable_and_apart(monkeypatch):
     with pytest.raises(ValueError, match="'preact' shares memory"):
         f(out[:4], x, w, preact=out[2:6], stream=fake.stream)
     f(out[:4], x, w, preact=out[4:], residual=out[:4], stream=fake.stream)  # in place, and a neighbour
+
+
+# ---------------------------------------------------------------- the choice of kernel
+def _near(values, step):
+    return sorted({max(step, int(v) // step * step) for v in values})
+
+
+@pytest.mark.parametrize("form", range(5))
+def test_every_choice_of_kernel_is_among_the_tested_shapes(form):
+    """Over a grid of sizes the rules choose no kernel, tile height or split
+    that the GPU tests' shapes do not reach as well."""
+    tested = {
+        C.BF16: C.FULL + C.PRODUCT, C.E4M3: C.FULL + C.PRODUCT_E4M3, C.GRADIENT: C.WEIGHTS,
+        C.GROUPED_BF16: C.GROUPS, C.GROUPED_E4M3: C.GROUPS_E4M3}[form]
+    step = 16 if form in (C.E4M3, C.GROUPED_E4M3) else 8
+    if form >= C.GROUPED_BF16:
+        covered = {C.choice(form, t, n, k, e) for e, t, n, k in tested}
+        reached = {C.choice(form, t, n, k, e) for e in (1, 2, 3, 8, 24, 64, 256, 1024)
+                   for t in (1, 2, 3, 7, 15, 30, 64, 100, 200, 500, 513, 8192)
+                   for n in (16, 128, 1000 // step * step, 4096) for k in (16, 320, 512, 1024, 2048, 14336)}
+    else:
+        covered = {C.choice(form, *s) for s in tested}
+        sizes = _near([8, 72, 136, 264, 400, 520, 656, 784, 1024, 1544, 2048, 2800, 4096, 5504, 8192, 14336], step)
+        rows = [1, 9, 16, 17, 32, 33, 50, 64, 65, 96, 128, 129, 200, 256, 400, 600, 800, 1200, 2000, 4096, 8192, 65536]
+        reached = {C.choice(form, m, n, k) for m in rows for n in sizes for k in sizes}
+    assert reached <= covered, reached - covered
+    assert len(reached) >= {C.BF16: 12, C.E4M3: 12, C.GRADIENT: 6}.get(form, 9)
+
+
+def test_the_choice_refuses_bad_sizes():
+    L = rt.lib()
+    x, y = ctypes.c_int(), ctypes.c_int()
+    for args in ((5, 4, 64, 64, 1, 148), (0, 0, 64, 64, 1, 148), (0, 4, 60, 64, 1, 148), (0, 4, 64, 64, 0, 148),
+                 (0, 4, 64, 64, 1, 1)):
+        assert L.thork_linear_choice(*args, ctypes.byref(x), ctypes.byref(y)) == rt.ERR_INVALID
+    assert L.thork_linear_choice(0, 4, 64, 64, 1, 148, None, ctypes.byref(y)) == rt.ERR_INVALID

@@ -179,24 +179,39 @@ double swap_us(int nkb, int m, int n, double mbytes, int sms, int bn, int split)
   return 5.1 + height * (0.32 * (split > 1 ? 1.3 : 1.0) + 0.02 * split) + (math > memory ? math : memory);
 }
 
+// A kernel and how it cuts the work: bn rows a tile and the contraction split
+// in `split` for swap_kernel, bn = 0 for rows_kernel or outer_kernel.
+struct Choice {
+  int bn, split;
+};
+
+// out[m, n] over nkb blocks of a contraction that moves mbytes.
+Choice by_estimate(int nkb, int m, int n, double mbytes, int sms, int least_bn) {
+  double best = rows_us(nkb, m, n, mbytes, sms / 2);
+  Choice choice = {0, 0};
+  for (int bn = least_bn; bn <= 128; bn *= 2)
+    for (int split = 1; split <= 8 && 2 * split <= nkb + 1; split *= 2) {
+      const double us = swap_us(nkb, m, n, mbytes, sms, bn, split);
+      if (us < best) {
+        best = us;
+        choice = {bn, split};
+      }
+    }
+  return choice;
+}
+
+Choice choose_dense(int elem, int m, int n, int k, int sms) {
+  const double mbytes =
+      (elem * (static_cast<double>(n) * k + static_cast<double>(m) * k) + 2.0 * m * n) * 1e-6;
+  return by_estimate(ceil_div(k, 128 / elem), m, n, mbytes, sms, 16);
+}
+
 template <int KIND, bool W_MN>
 int dense_product(const Product &p, const GemmArgs &g, cudaStream_t s, const char *what) {
   int rc, sms;
   if ((rc = thork_sm_count(&sms))) return rc;
-  const int elem = KIND == KIND_BF16 ? 2 : 1, nkb = ceil_div(p.k, 128 / elem);
-  const double mbytes = (elem * (static_cast<double>(p.n) * p.k + static_cast<double>(p.rows) * p.k) +
-                         2.0 * p.rows * p.n) * 1e-6;
-  double best = rows_us(nkb, p.rows, p.n, mbytes, sms / 2);
-  int bn = 0, split = 0;
-  for (int b = 16; b <= 128; b *= 2)
-    for (int c = 1; c <= 8 && 2 * c <= nkb + 1; c *= 2) {
-      const double us = swap_us(nkb, p.rows, p.n, mbytes, sms, b, c);
-      if (us < best) {
-        best = us;
-        bn = b;
-        split = c;
-      }
-    }
+  const Choice c = choose_dense(KIND == KIND_BF16 ? 2 : 1, p.rows, p.n, p.k, sms);
+  const int bn = c.bn, split = c.split;
   switch (bn) {
     case 16: return swap_product<KIND, 16, 6, W_MN, false>(p, g, split, s, what);
     case 32: return swap_product<KIND, 32, 5, W_MN, false>(p, g, split, s, what);
@@ -213,19 +228,25 @@ int dense_product(const Product &p, const GemmArgs &g, cudaStream_t s, const cha
 // 4096 126 against 131 with rows_kernel; E=52 of 1432 x 2416 50 / 55; E=64 of
 // 2048 x 2048 86 / 85; E=37 of 760 x 1304 28.6 / 22.3; e4m3 E=64 of 2048 x
 // 1024 48 / 35).
+Choice choose_grouped(int elem, int groups, int rows, int n, int k, int sms) {
+  const int mean = ceil_div(rows, groups);
+  if (mean > 24 || rows > 512) return {0, 0};
+  // two CTAs fit on an SM: split the contraction until they are all in use
+  const long long held = groups < rows ? groups : rows;
+  const int nkb = ceil_div(k, 128 / elem);
+  int split = 1;
+  while (split < 8 && 2 * split * held * ceil_div(n, 128) <= 2 * sms && 4 * split <= nkb) split *= 2;
+  return {mean <= 4 ? 16 : 32, split};
+}
+
 template <int KIND, bool W_MN>
 int grouped_product(const Product &p, const GemmArgs &g, cudaStream_t s, const char *what) {
   int rc, sms;
   if ((rc = thork_sm_count(&sms))) return rc;
-  const int mean = ceil_div(p.rows, p.groups);
-  if (mean > 24 || p.rows > 512) return rows_product<KIND, W_MN, true>(p, g, s, what);
-  // two CTAs fit on an SM: split the contraction until they are all in use
-  const long long held = p.groups < p.rows ? p.groups : p.rows;
-  const int nkb = ceil_div(p.k, KIND == KIND_BF16 ? 64 : 128);
-  int split = 1;
-  while (split < 8 && 2 * split * held * ceil_div(p.n, 128) <= 2 * sms && 4 * split <= nkb) split *= 2;
-  if (mean <= 4) return swap_product<KIND, 16, 5, W_MN, true>(p, g, split, s, what);
-  return swap_product<KIND, 32, 5, W_MN, true>(p, g, split, s, what);
+  const Choice c = choose_grouped(KIND == KIND_BF16 ? 2 : 1, p.groups, p.rows, p.n, p.k, sms);
+  if (c.bn == 16) return swap_product<KIND, 16, 5, W_MN, true>(p, g, c.split, s, what);
+  if (c.bn == 32) return swap_product<KIND, 32, 5, W_MN, true>(p, g, c.split, s, what);
+  return rows_product<KIND, W_MN, true>(p, g, s, what);
 }
 
 // The dense weight gradient by swap_kernel: 128 columns n by BN rows k a
@@ -276,25 +297,18 @@ int weight_gradient(const void *x, const void *dy, int rows, int n, int k, const
 // estimates of dense_product (us, outer_kernel / swap_kernel: 2604 rows of 184
 // x 152 17.0 / 7.7, 8054 of 256 x 536 32.3 / 12.6, 8192 of 1024 x 1024 30.9 /
 // 22.7; 637 of 1800 x 488 8.5 / 10.7, 7008 of 2168 x 1384 53 / 96).
+Choice choose_gradient(int rows, int n, int k, int sms) {
+  const double mbytes = 2e-6 * (static_cast<double>(n) * k + static_cast<double>(rows) * (n + k));
+  return by_estimate(ceil_div(rows, 64), k, n, mbytes, sms, 64);
+}
+
 int dense_gradient(const void *x, const void *dy, int rows, int n, int k, const GemmArgs &g, cudaStream_t s,
                    const char *what) {
   int rc, sms;
   if ((rc = thork_sm_count(&sms))) return rc;
-  const int nkb = ceil_div(rows, 64);
-  const double mbytes = 2e-6 * (static_cast<double>(n) * k + static_cast<double>(rows) * (n + k));
-  double best = rows_us(nkb, k, n, mbytes, sms / 2);
-  int bn = 0, split = 0;
-  for (int b = 64; b <= 128; b *= 2)
-    for (int c = 1; c <= 8 && 2 * c <= nkb + 1; c *= 2) {
-      const double us = swap_us(nkb, k, n, mbytes, sms, b, c);
-      if (us < best) {
-        best = us;
-        bn = b;
-        split = c;
-      }
-    }
-  if (bn == 64) return swap_gradient<64, 4>(x, dy, rows, n, k, g, split, s, what);
-  if (bn == 128) return swap_gradient<128, 3>(x, dy, rows, n, k, g, split, s, what);
+  const Choice c = choose_gradient(rows, n, k, sms);
+  if (c.bn == 64) return swap_gradient<64, 4>(x, dy, rows, n, k, g, c.split, s, what);
+  if (c.bn == 128) return swap_gradient<128, 3>(x, dy, rows, n, k, g, c.split, s, what);
   return weight_gradient<false>(x, dy, rows, n, k, g, s, what);
 }
 
@@ -505,6 +519,27 @@ int backward(void *da, void *db, float *dbias, const void *dout, const void *a, 
   return THORK_OK;
 }
 }  // namespace
+
+extern "C" int thork_linear_choice(int form, int M, int N, int K, int E, int sms, int *tile_rows,
+                                   int *split) {
+  const char *what = "linear_choice";
+  int rc;
+  if (!tile_rows || !split) return thork_set_error(THORK_ERR_INVALID, "%s: NULL output", what);
+  if ((rc = check_sizes(M, N, K, 8, what))) return rc;
+  if (sms < 2 || E < 1) return thork_set_error(THORK_ERR_INVALID, "%s: sms=%d E=%d", what, sms, E);
+  Choice c;
+  switch (form) {
+    case THORK_CHOICE_BF16: c = choose_dense(2, M, N, K, sms); break;
+    case THORK_CHOICE_E4M3: c = choose_dense(1, M, N, K, sms); break;
+    case THORK_CHOICE_GRADIENT: c = choose_gradient(M, N, K, sms); break;
+    case THORK_CHOICE_GROUPED_BF16: c = choose_grouped(2, E, M, N, K, sms); break;
+    case THORK_CHOICE_GROUPED_E4M3: c = choose_grouped(1, E, M, N, K, sms); break;
+    default: return thork_set_error(THORK_ERR_INVALID, "%s: unknown form %d", what, form);
+  }
+  *tile_rows = c.bn;
+  *split = c.split;
+  return THORK_OK;
+}
 
 extern "C" int thork_linear_bf16(const void *d_a, const void *d_b, void *d_out, const void *d_bias,
                                  const void *d_residual, void *d_preact, int M, int N, int K,

@@ -108,6 +108,7 @@ _SIGNATURES = {
     "thork_gemm_bf16_allgather_mc": [_vp, _vp, _vp, _i, _i, _i, _i, _vp],
     "thork_gemm_e4m3_allgather_mc": [_vp, _vp, _vp, _i, _i, _i, _i, ctypes.c_float,
                                      ctypes.c_float, _vp],
+    "thork_linear_choice": [_i] * 6 + [ctypes.POINTER(_i)] * 2,
     "thork_linear_bf16": [_vp] * 6 + [_i] * 5 + [_vp],
     "thork_linear_e4m3": [_vp] * 6 + [_i] * 3 + [ctypes.c_float] * 2 + [_i] * 2 + [_vp],
     "thork_linear_backward_bf16": [_vp] * 8 + [_i] * 4 + [_vp],
