@@ -182,8 +182,9 @@ THORK_API int thork_tensor_map_2d(void *out128, int dtype, const void *d_base,
  * wait gives up (code in bits 0-7, site in bits 8-15).  No reference
  * counterpart (the reference has no bounded waits).                       */
 THORK_API int thork_kernel_status(unsigned *status, int clear);
-/* Waits for `stream` and returns the status word as it is then, without
- * clearing it or waiting for other streams.                                */
+/* Waits for `stream` and returns what the linear-layer operators' kernels
+ * have reported on the current device, without clearing it or waiting for
+ * other streams.  thork_kernel_status includes it.                         */
 THORK_API int thork_stream_status(unsigned *status, void *stream);
 /* Device address of the current device's status word, passed to traced tile
  * kernels as their hidden last parameter.                                  */

@@ -100,28 +100,37 @@ def test_the_longest_contraction_of_a_gradient():
         _all_of_it(db)
 
 
-def test_a_status_that_says_a_wait_expired_is_raised():
-    """A status planted in the device's word, as a kernel leaves it whose wait
-    expired: asynchronous calls leave it there, the next call that
-    synchronises raises it and clears it; its own output is as ever."""
-    m, n, k = 5, 264, 136
+def _stream_status(stream):
+    v = ctypes.c_uint(0)
+    rt.check(rt.lib().thork_stream_status(ctypes.byref(v), stream.handle))
+    return v.value
+
+
+@pytest.mark.parametrize("t", [40, 600])
+def test_what_a_kernel_reports_is_read_behind_its_stream(t):
+    """The operators report to a word of their own, which a call that
+    synchronises looks at (wrong offsets stay in it, an expired wait is
+    raised); kernel_status shows and clears it."""
+    e, n, k = 4, 136, 72
     rng = np.random.default_rng(2)
-    a, b = bits(rng, m, k), bits(rng, k, n, std=0.1)
-    want, out = np.zeros((m, n), np.uint16), np.zeros((m, n), np.uint16)
-    f = tk.kernels.linear(m, n, k)
-    f(want, a, b)
-    A, B, O = rt.to_device(a), rt.to_device(b), rt.empty((m, n), np.uint16)
+    A, B, out = rt.to_device(bits(rng, t, k)), rt.to_device(bits(rng, e, k, n)), rt.empty((t, n), np.uint16)
+    good = rt.to_device(np.array([0, 10, 10, 30, t], np.int32))
+    bad = rt.to_device(np.array([0, 10, 7, 30, 5 * t], np.int32))
+    f = tk.kernels.grouped_matmul(e, t, n, k)
     s = rt.Stream()
-    word = np.array([1 | 0x53 << 8], np.uint32)
-    for call in (lambda: f(O, A, B, stream=s), lambda: f(out, a, b, stream=s, sync=False)):
-        rt.copy_htod(rt.status_pointer(), word)
-        f(O, A, B, stream=s, sync=False)
-        with pytest.raises(rt.CudaError, match="bounded wait expired at site 83"):
-            call()
-        assert rt.kernel_status() == 0
-        np.testing.assert_array_equal(O.to_host(), want)
-    f(out, a, b)
-    np.testing.assert_array_equal(out, want)
+    f(out, A, B, good, stream=s, sync=False)
+    assert _stream_status(s) == 0
+    f(out, A, B, bad, stream=s, sync=False)
+    assert _stream_status(s) == 2 | 0x40 << 8
+    f(out, A, B, good, stream=s)
+    assert rt.kernel_status(clear=False) == 2 | 0x40 << 8
+    assert rt.kernel_status() == 2 | 0x40 << 8
+    assert rt.kernel_status() == 0 and _stream_status(s) == 0
+    # a word planted on the device, as another kernel's expired wait leaves it,
+    # is that kernel's caller's to read
+    rt.copy_htod(rt.status_pointer(), np.array([1 | 0x14 << 8], np.uint32))
+    f(out, A, B, good, stream=s)
+    assert rt.kernel_status() == 1 | 0x14 << 8
 
 
 @pytest.mark.parametrize("which", ["linear ragged 777", "linear backward 200", "grouped backward odd"])

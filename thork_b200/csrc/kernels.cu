@@ -24,6 +24,7 @@ namespace {
 constexpr int kMaxDevices = 64;
 std::mutex g_dev_mu;
 unsigned *g_status[kMaxDevices] = {};
+unsigned *g_host_status[kMaxDevices] = {};  // see thork_host_status_word
 int g_sms[kMaxDevices] = {};
 uint64_t g_smem_set[kMaxDevices] = {};  // bit i: kernel i has its smem attribute set
 
@@ -49,6 +50,22 @@ int thork_status_word(unsigned **d_status) {
     g_status[dev] = static_cast<unsigned *>(p);
   }
   *d_status = g_status[dev];
+  return THORK_OK;
+}
+
+int thork_host_status_word(unsigned **word) {
+  int dev, rc;
+  if ((rc = current_device(&dev))) return rc;
+  std::lock_guard<std::mutex> lk(g_dev_mu);
+  if (!g_host_status[dev]) {
+    void *p = nullptr;
+    // one address for both sides (unified addressing)
+    cudaError_t e = cudaHostAlloc(&p, 16, cudaHostAllocMapped | cudaHostAllocPortable);
+    if (e != cudaSuccess) return thork_cuda_error(e, "cudaHostAlloc(status word)");
+    g_host_status[dev] = static_cast<unsigned *>(p);
+    *g_host_status[dev] = 0;
+  }
+  *word = g_host_status[dev];
   return THORK_OK;
 }
 
@@ -79,14 +96,16 @@ static int ensure_smem(const void *kernel, int kernel_id, int bytes) {
 
 extern "C" int thork_kernel_status(unsigned *status, int clear) {
   if (!status) return thork_set_error(THORK_ERR_INVALID, "status is NULL");
-  unsigned *d;
-  int rc = thork_status_word(&d);
-  if (rc) return rc;
+  unsigned *d, *h;
+  int rc;
+  if ((rc = thork_status_word(&d)) || (rc = thork_host_status_word(&h))) return rc;
   cudaError_t e = cudaDeviceSynchronize();
   if (e != cudaSuccess) return thork_cuda_error(e, "cudaDeviceSynchronize");
   e = cudaMemcpy(status, d, sizeof(unsigned), cudaMemcpyDeviceToHost);
   if (e != cudaSuccess) return thork_cuda_error(e, "read status word");
+  *status |= *static_cast<volatile unsigned *>(h);
   if (clear) {
+    *static_cast<volatile unsigned *>(h) = 0;
     e = cudaMemset(d, 0, 16);
     if (e != cudaSuccess) return thork_cuda_error(e, "clear status word");
   }
@@ -95,14 +114,12 @@ extern "C" int thork_kernel_status(unsigned *status, int clear) {
 
 extern "C" int thork_stream_status(unsigned *status, void *stream) {
   if (!status) return thork_set_error(THORK_ERR_INVALID, "status is NULL");
-  unsigned *d;
-  int rc = thork_status_word(&d);
+  unsigned *h;
+  int rc = thork_host_status_word(&h);
   if (rc) return rc;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  cudaError_t e = cudaMemcpyAsync(status, d, sizeof(unsigned), cudaMemcpyDeviceToHost, s);
-  if (e != cudaSuccess) return thork_cuda_error(e, "read status word");
-  e = cudaStreamSynchronize(s);
+  cudaError_t e = cudaStreamSynchronize(static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return thork_cuda_error(e, "cudaStreamSynchronize");
+  *status = *static_cast<volatile unsigned *>(h);
   return THORK_OK;
 }
 

@@ -423,7 +423,7 @@ int linear(const void *a, const void *b, void *c, const void *bias, const void *
   g.epi = {static_cast<unsigned short *>(c), static_cast<unsigned short *>(preact),
            static_cast<const unsigned short *>(bias), static_cast<const unsigned short *>(residual),
            nullptr, alpha, act, N, nullptr};
-  if ((rc = thork_status_word(&g.epi.status))) return rc;
+  if ((rc = thork_host_status_word(&g.epi.status))) return rc;
   g.GM = g.rows = M;
   g.GN = N;
   g.GK = K;
@@ -450,7 +450,7 @@ int grouped(const void *a, const void *b, void *c, const int *offsets, void *pre
   GemmArgs g = {};
   g.epi = {static_cast<unsigned short *>(c), static_cast<unsigned short *>(preact), nullptr, nullptr,
            group_scale, alpha, act, N, nullptr};
-  if ((rc = thork_status_word(&g.epi.status))) return rc;
+  if ((rc = thork_host_status_word(&g.epi.status))) return rc;
   g.GM = g.rows = T;
   g.GN = N;
   g.GK = K;
@@ -488,7 +488,7 @@ int backward(void *da, void *db, float *dbias, const void *dout, const void *a, 
   const void *dz = bent ? dpre : dout;
   GemmArgs g = {};
   g.epi.alpha = 1.0f;
-  if ((rc = thork_status_word(&g.epi.status))) return rc;
+  if ((rc = thork_host_status_word(&g.epi.status))) return rc;
   g.rows = rows;
   g.offsets = offsets;
   g.groups = groups;

@@ -15,6 +15,11 @@ int thork_encode_tmap_3d(void *out128, int dtype, const void *base, uint64_t d0,
                          uint32_t box0, uint32_t box1);
 // Per-device status word (4 x u32, cudaMalloc'd and zeroed on first use).
 int thork_status_word(unsigned **d_status);
+// The linear-layer operators' status word, one per device in page-locked host
+// memory that kernels write when something went wrong: the host reads it after
+// a wait for the stream without a copy (a synchronising linear of 16 x 4096 x
+// 4096 took 19.7 us without a read, 28-29 with one of a word on the device).
+int thork_host_status_word(unsigned **word);
 // Cached multiprocessor count of the current device.
 int thork_sm_count(int *n);
 // Pipelined copies through pinned slots for pageable host memory (staging.cu).

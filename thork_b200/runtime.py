@@ -248,8 +248,9 @@ def check_kernel_status(what: str) -> None:
 
 
 def finish_stream(stream: "Stream", what: str) -> None:
-    """Wait for ``stream`` and raise if a bounded wait has expired, in this
-    call's kernels or in ones queued earlier whose status nobody has read."""
+    """Wait for ``stream`` and raise if a bounded wait of a linear-layer
+    operator has expired, in this call or in an earlier one whose status
+    nobody has read."""
     v = ctypes.c_uint(0)
     check(lib().thork_stream_status(ctypes.byref(v), stream.handle), what)
     if v.value & 1:
