@@ -293,3 +293,49 @@ def test_host_memory_is_not_wrapped():
                                   np.arange(16, 64))
     d = rt.to_device(host)
     assert rt.wrap_pointer(d.ptr, (64,), np.uint16).ptr == d.ptr
+
+
+def test_two_threads_with_streams_of_their_own():
+    """Forward, backward and grouped calls of the same handles from two threads
+    at once, each on its own stream and arrays, repeat the calls of one."""
+    import threading
+
+    t, n, k, e = 300, 264, 520, 3
+    rng = np.random.default_rng(5)
+    host = dict(a=bits(rng, t, k), b=bits(rng, k, n, std=0.05), w=bits(rng, e, k, n, std=0.05),
+                dout=bits(rng, t, n, std=0.1), off=np.array([0, 100, 117, 290], np.int32))
+    L = tk.kernels
+    fwd, bwd = L.linear(t, n, k, activation="gelu"), L.linear_backward(t, n, k, activation="gelu")
+    few = L.linear(7, n, k, activation="silu", static_weights=True)
+    grp, grp_b = L.grouped_matmul(e, t, n, k), L.grouped_matmul_backward(e, t, n, k)
+
+    def work(times, results):
+        D = {name: rt.to_device(x) for name, x in host.items()}
+        z, dz, out, gout = (rt.empty((t, n), np.uint16) for _ in range(4))
+        small, x7 = rt.empty((7, n), np.uint16), rt.to_device(host["a"][:7])
+        da, db, dw = rt.empty((t, k), np.uint16), rt.empty((k, n), np.uint16), rt.empty((e, k, n), np.uint16)
+        dbias = rt.empty((n,), np.float32)
+        gout.zero()
+        s = rt.Stream()
+        rt.synchronize()
+        kw = dict(stream=s, sync=False)
+        for _ in range(times):
+            fwd(out, D["a"], D["b"], preact=z, **kw)
+            few(small, x7, D["b"], **kw)
+            bwd(da, db, dbias, D["dout"], D["a"], D["b"], z, dz, **kw)
+            grp(gout, D["a"], D["w"], D["off"], **kw)
+            grp_b(None, dw, D["dout"], D["a"], None, D["off"], **kw)
+        s.synchronize()
+        results.append([x.to_host(stream=s) for x in (out, z, small, da, db, dbias, dz, gout, dw)])
+
+    want, got = [], []
+    work(1, want)
+    threads = [threading.Thread(target=work, args=(40, got)) for _ in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert len(got) == 2
+    for result in got:
+        for x, y in zip(result, want[0]):
+            np.testing.assert_array_equal(x, y)
