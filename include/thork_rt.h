@@ -351,7 +351,8 @@ enum {
 };
 /* B is written by no kernel launched earlier on the stream (decode weights):
  * products of few rows then start fetching it before the previous kernel
- * has finished.  The others ignore the flag.                               */
+ * has finished.  Other products ignore the flag, and so do grouped ones,
+ * whose tiles know their group's weights only from `offsets`.              */
 #define THORK_LINEAR_W_STATIC 1
 
 /* z = A[M,K] . B[K,N] + bias[N];  out = act(z) + residual[M,N].

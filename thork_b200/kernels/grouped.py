@@ -36,9 +36,12 @@ class grouped_matmul:
 
     With ``dtype=tk.dt.float8_e4m3`` the call takes ``scale_a`` (a number) and
     ``scale_b`` (float32 ``[E]``, one per expert, or ``None`` for ones):
-    ``z[r] = scale_a * scale_b[e] * (A[r] @ B[e])``.  ``activation``,
-    ``preact`` and ``static_weights`` are as for ``tk.kernels.linear``.  K is
-    at most 2^23.
+    ``z[r] = scale_a * scale_b[e] * (A[r] @ B[e])``.  ``activation`` and
+    ``preact`` are as for ``tk.kernels.linear``.  K is at most 2^23.
+
+    ``static_weights`` may be given as to ``tk.kernels.linear`` and changes
+    nothing: which expert's weights a tile needs is known only when the
+    previous kernel, which may write ``offsets``, has finished.
     """
 
     name = "grouped_matmul"
