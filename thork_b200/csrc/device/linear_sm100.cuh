@@ -169,8 +169,8 @@ __device__ __forceinline__ float bf16_hi(u32 w) { return __uint_as_float(w & 0xF
 //
 // Two values at a time, in the packed fp32 instructions: slope_kernel has
 // about as many instructions to issue as bytes to move (4096 x 14336, gelu:
-// 126 us with erff and expf, 73 with the approximation, 65-70 packed; its
-// traffic takes 54).
+// 126 us with erff and expf, 73 with an approximation of its own, 62-70 packed;
+// its traffic takes 54).
 struct F2 {
   u64 v;
 };
@@ -357,8 +357,8 @@ __device__ __forceinline__ void scan_groups(const int *offsets, int groups, int 
 // [128 r, 128 r + 128)), the rows its N dimension (CTA r holds one half of the
 // tile's rows).  The N dimension of an instruction may be any multiple of 32,
 // so a tile has as many rows as there are, in units of 64: a group's rows, or
-// a product's, are dealt out in even tiles of at most four units, and no
-// multiplication is spent on rows of another group.  With rows as the M
+// a product's, fill tiles of four units and leave the rest to a last, shorter
+// one, and no multiplication is spent on rows of another group.  With rows as the M
 // dimension every group would round up to 256 rows.
 //
 // Persistent: pair i takes tiles i, i + pairs, ...; the tiles of the last,
@@ -369,9 +369,14 @@ __device__ __forceinline__ void scan_groups(const int *offsets, int groups, int 
 // per TMEM lane quadrant, taking the tile's 32-row slices in turn.
 //
 // Bound by the tensor pipe (90 % of active cycles at 4096 x 4096 x 14336), and
-// back to back by the power cap.  Measured: 4096^3 91 us (1508 TFLOP/s), 8192^3
-// 695 us (1583) in bursts, 832 us (1322) over 1.5 s; e4m3 8192^3 334 us alone;
-// 8 experts of 14336 x 4096 with 8192 rows 651 us alone (1478).  Six stages of
+// back to back by the power cap.  Ten calls after a pause / 1.5 s back to back:
+// 4096^3 94 us (1460 TFLOP/s) / 110 (1248), with gelu, bias, residual and saved
+// pre-activation 103 (1337) / 122 (1130); 8192^3 732 (1502) / 829 (1326); e4m3
+// 8192^3 with bias, relu and residual 396 (2776) / 443 (2484); 8 experts of 14336
+// x 4096 with 8192 rows and silu 655 (1468) / 736 (1307), 725 / 826 with the rows
+// dealt out unevenly.  Where tiles are fewer than pairs, splitting them by rows
+// fills the pairs but shortens no tile's contraction, of which a block takes 0.2
+// to 0.3 us however few its rows: 256 x 4096 x 4096 22 us of 5.8.  Six stages of
 // 32 KiB per CTA; 512-column tiles of four 48 KiB stages gained 1 % at 8192^3
 // and lost 3 % at 4096^3.
 template <int KIND_, bool W_MN_, bool GROUPED_>
@@ -899,9 +904,10 @@ __global__ void __launch_bounds__(C::THREADS, 1)
 // TMA, in whole 128-byte lines; it clips what lies outside dW.
 //
 // Bound by the tensor pipe for many rows (4096 x 4096 x 14336: 95 % of active
-// cycles, 311 us, 1545 TFLOP/s), by the operands' latency for groups of a few
-// hundred (8 x 512 rows of 4096 x 4096: 119 us) and by the writes of dW below
-// (64 x 64 rows of 4096 x 1024: 114 us, 4.7 TB/s; 16-byte stores took 286).
+// cycles, 328 us or 1465 TFLOP/s after a pause, 377 or 1277 back to back), by the
+// operands' latency for groups of a few hundred (8 x 512 rows of 4096 x 4096: 120
+// us) and by the writes of dW below (64 x 64 rows of 4096 x 1024: 117 us, 4.6
+// TB/s; 16-byte stores took 286).
 template <bool GROUPED_>
 struct OuterCfg {
   static constexpr bool GROUPED = GROUPED_;
@@ -1317,9 +1323,10 @@ __global__ void __launch_bounds__(C::THREADS, 1)
 // finished pipeline stages, and each CTA sums every S-th row over the cluster
 // in rank order (deterministic, no workspace in global memory) and stores it.
 //
-// Bound by the weights' bytes: 1 x 14336 x 4096 20.8 us (5.6 TB/s, S=2), 16 x
-// 4096 x 14336 21.5 us (5.5 TB/s, S=8); 128 x 4096 x 4096 14.7 us.  5 to 6
-// stages leave room for two CTAs an SM and hold 190 KiB of loads in flight.
+// Bound by the weights' bytes: 1 x 14336 x 4096 21.0 us (5.6 TB/s, S=2), 16 x
+// 4096 x 14336 21.7 us (5.4 TB/s, S=8).  Of narrower weights by some 5 us that
+// are fixed (launch, first loads, sum): 1 x 4096 x 4096 9.2 us of 5.1, 128 x
+// 4096 x 4096 14.4 of 5.5.  5 to 6 stages leave room for two CTAs an SM and hold 190 KiB of loads in flight.
 //
 // X_MN: X is given as its transpose, [k, m] row-major.  That is the weights'
 // gradient, out[k, n] = sum over rows X[row, k] dY[row, n], where it has few
@@ -1624,8 +1631,8 @@ __global__ void __launch_bounds__(C::THREADS)
 // that the blocks fill the GPU.
 //
 // Bound by its traffic, with about as many instructions to issue: 4096 x 14336
-// with gelu and the sums 65-70 us (5.0-5.4 TB/s), 4096 x 4096 with silu 17 us
-// (5.9 TB/s).
+// with gelu and the sums 62-70 us (5.0-5.6 TB/s), 4096 x 4096 with silu 18-20 us
+// (5.1-5.6 TB/s).
 struct SlopeArgs {
   const unsigned short *dout, *preact;
   unsigned short *dpre;

@@ -138,15 +138,28 @@ int rows_product(const Product &p, const GemmArgs &g, cudaStream_t s, const char
 
 // ---------------------------------------------------------------- choice of kernel
 // Microseconds of one dense product by each kernel, estimated.  The forms and
-// constants were fitted to 4050 products timed on B200 with every choice (M 1
-// to 1600, N and K 128 to 14336, bf16); picking by them is 1 % (mean) from the
-// best choice of each beyond the timing's noise.  Some of the sides, measured
-// (us; swap_kernel with BN rows a tile and the contraction split in S):
-//     M    N     K    rows  swap (BN/S)      M    N     K    rows  swap (BN/S)
-//     1  4096  4096   18.7   10.8 (16/4)    256  4096  4096   19.4   17.0 (128/4)
-//    64  1544  1032    8.8    6.8 (32/4)    256 14336  4096   29.4   40.0 (128/1)
-//   128  4096  4096   19.2   13.4 (64/4)    512   512  8192   32.7   15.3 (128/8)
-//   128 14336  4096   25.1   30.1 (128/2)   777  1544  1032   10.6   14.5 (128/2)
+// constants were fitted to timings of 4050 bf16 products on B200 (M 1 to 1600, N
+// and K 128 to 14336), each with the choices that looked possible: on the 3537
+// whose choice by the estimates was among them it is 1.9 % (mean) from the best,
+// on 6.7 % of them by more than 10 %, at worst 1.68 times.  e4m3 products take
+// the same estimates with their own blocks and bytes.  Both sides, every choice
+// timed (us; floor: bytes or operations at the measured rates; swap_kernel's best
+// with BN rows a tile and the contraction split in S, behind it the rule's):
+//                        bf16                                  e4m3
+//     M    N     K   floor  rows  swap  (BN/S)  rule     floor  rows  swap  (BN/S)  rule
+//     1  4096  4096   5.1   19.1   9.1   32/8   16/8      2.6   11.6   7.1   16/8   16/8
+//    64  4096  4096   5.3   19.6  11.7   64/8   64/8      2.7   12.0   8.8   32/4   64/8
+//   128  4096  4096   5.5   21.1  14.0   64/4  128/8      2.8   12.4  10.3   64/4   64/4
+//   256  4096  4096   5.8   22.0  18.0  128/4   rows      3.0   12.8  13.4   64/2   rows
+//    64 14336  4096  18.3   23.3  25.2   64/2   rows      9.3   14.0  16.7   32/1   rows
+//   256 14336  4096  19.4   29.7  41.1  128/1   rows     10.3   18.5  25.8  128/1   rows
+//    64  4096 14336  18.3   55.3  24.1   64/8   64/8      9.2   29.7  15.5   64/8   64/8
+//   256  4096 14336  19.4   58.5  36.3  128/4  128/4      9.9   31.5  22.6  128/4  128/4
+//   400  4096 14336  28.7   64.4  60.5  128/2   rows     14.4   34.7  36.0  128/2   rows
+//   128  1552  1040   0.6    8.9   6.8   32/4   32/4      0.3    6.9   5.5   16/1   32/4
+//   777  1552  1040   1.5   10.0  13.1   64/1   rows      0.8    8.1  10.6   64/1   rows
+// Of 28 products of either type (these and their neighbours at 1 to 777 rows) the
+// rule is within 10 % of the best on all but 256 x 4096 x 4096 in bf16.
 constexpr int ceil_div(long long a, int b) { return static_cast<int>((a + b - 1) / b); }
 
 double rows_us(int nkb, int m, int n, double mbytes, int pairs) {
@@ -294,9 +307,10 @@ int weight_gradient(const void *x, const void *dy, int rows, int n, int k, const
 }
 
 // Few tiles with many rows to sum over: split the rows over clusters, by the
-// estimates of dense_product (us, outer_kernel / swap_kernel: 2604 rows of 184
-// x 152 17.0 / 7.7, 8054 of 256 x 536 32.3 / 12.6, 8192 of 1024 x 1024 30.9 /
-// 22.7; 637 of 1800 x 488 8.5 / 10.7, 7008 of 2168 x 1384 53 / 96).
+// same estimates (us, outer_kernel / swap_kernel: 2604 rows of 184 x 152 17.0 /
+// 7.7, 8054 of 256 x 536 33.6 / 12.9, 8192 of 1024 x 1024 33.7 / 22.9; 637 of
+// 1800 x 488 8.7 / 10.9, 7008 of 2168 x 1384 56 / 90; of those timed the rule
+// missed one, 1000 of 776 x 520, with 9.8 / 8.9).
 Choice choose_gradient(int rows, int n, int k, int sms) {
   const double mbytes = 2e-6 * (static_cast<double>(n) * k + static_cast<double>(rows) * (n + k));
   return by_estimate(ceil_div(rows, 64), k, n, mbytes, sms, 64);
