@@ -125,8 +125,12 @@ def test_an_expired_wait_is_raised_by_calls_that_synchronise(monkeypatch):
         f(out, a, b, stream=fake.stream)
     assert e.value.code == rt.ERR_KERNEL and fake.status == 0  # raised once
     f(out, a, b, stream=fake.stream)
-    # host arrays: the call synchronises in any case
+    # another thread's call that cleared the word in between
     fake.status = expired
+    monkeypatch.setattr(rt, "kernel_status", lambda clear=True: 0)
+    with pytest.raises(rt.CudaError, match="bounded wait expired at site 83"):
+        f(out, a, b, stream=fake.stream)
+    # host arrays: the call synchronises in any case
     host = np.zeros((4, 64), np.uint16)
     with pytest.raises(rt.CudaError, match="bounded wait"):
         f(host, a, b, stream=fake.stream, sync=False)

@@ -239,12 +239,16 @@ def kernel_status(clear: bool = True) -> int:
     return v.value
 
 
+def _raise_status(st: int, what: str) -> None:
+    raise CudaError(
+        f"kernel {what} reported status 0x{st:x} (a bounded wait expired at site "
+        f"{(st >> 8) & 0xFF})", ERR_KERNEL)
+
+
 def check_kernel_status(what: str) -> None:
     st = kernel_status(clear=True)
     if st:
-        raise CudaError(
-            f"kernel {what} reported status 0x{st:x} (a bounded wait expired at site "
-            f"{(st >> 8) & 0xFF})", ERR_KERNEL)
+        _raise_status(st, what)
 
 
 def finish_stream(stream: "Stream", what: str) -> None:
@@ -254,7 +258,8 @@ def finish_stream(stream: "Stream", what: str) -> None:
     v = ctypes.c_uint(0)
     check(lib().thork_stream_status(ctypes.byref(v), stream.handle), what)
     if v.value & 1:
-        check_kernel_status(what)
+        kernel_status(clear=True)
+        _raise_status(v.value, what)  # whoever else has cleared it meanwhile
 
 
 # --------------------------------------------------------------------------
