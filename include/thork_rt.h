@@ -187,7 +187,8 @@ THORK_API int thork_kernel_status(unsigned *status, int clear);
  * other streams.  thork_kernel_status includes it.                         */
 THORK_API int thork_stream_status(unsigned *status, void *stream);
 /* Device address of the current device's status word, passed to traced tile
- * kernels as their hidden last parameter.                                  */
+ * kernels as their hidden last parameter.  The linear-layer operators report
+ * to a word of their own (thork_stream_status).                            */
 THORK_API int thork_status_pointer(void **d_status);
 
 /* ---- library kernels --------------------------------------------------

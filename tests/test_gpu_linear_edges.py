@@ -339,3 +339,32 @@ def test_two_threads_with_streams_of_their_own():
     for result in got:
         for x, y in zip(result, want[0]):
             np.testing.assert_array_equal(x, y)
+
+
+def test_a_first_call_that_is_captured():
+    """In a process whose library has been used otherwise before, an operator's
+    first call may be one that is captured: it allocates nothing."""
+    import os
+    import subprocess
+    import sys
+
+    pytest.importorskip("torch")
+    code = """
+import numpy as np, torch, thork_b200 as tk
+rt = tk.runtime
+rt.status_pointer()
+A, B, O = (torch.randn(64, 64, device="cuda").bfloat16() for _ in range(3))
+a, b, o = (rt.wrap_pointer(t.data_ptr(), (64, 64), np.uint16, owner=t) for t in (A, B, O))
+f, graph = tk.kernels.linear(64, 64, 64), torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    f(o, a, b, stream=rt.Stream.from_handle(torch.cuda.current_stream().cuda_stream), sync=False)
+O.zero_()
+graph.replay()
+torch.cuda.synchronize()
+first = O.clone()
+f(o, a, b)
+assert torch.equal(first, O) and O.any() and rt.kernel_status() == 0
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr

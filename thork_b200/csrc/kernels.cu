@@ -37,34 +37,41 @@ int current_device(int *dev) {
 }
 }  // namespace
 
-int thork_status_word(unsigned **d_status) {
-  int dev, rc;
-  if ((rc = current_device(&dev))) return rc;
+// Both words of a device are allocated together, so that whichever call of the
+// library came first, no later one allocates (a stream capture forbids it).
+static int status_words(int *dev) {
+  int rc;
+  if ((rc = current_device(dev))) return rc;
   std::lock_guard<std::mutex> lk(g_dev_mu);
-  if (!g_status[dev]) {
+  if (!g_status[*dev]) {
     void *p = nullptr;
     cudaError_t e = cudaMalloc(&p, 16);
     if (e != cudaSuccess) return thork_cuda_error(e, "cudaMalloc(status word)");
     e = cudaMemset(p, 0, 16);
     if (e != cudaSuccess) return thork_cuda_error(e, "cudaMemset(status word)");
-    g_status[dev] = static_cast<unsigned *>(p);
+    g_status[*dev] = static_cast<unsigned *>(p);
   }
+  if (!g_host_status[*dev]) {
+    void *p = nullptr;
+    // one address for both sides (unified addressing)
+    cudaError_t e = cudaHostAlloc(&p, 16, cudaHostAllocMapped | cudaHostAllocPortable);
+    if (e != cudaSuccess) return thork_cuda_error(e, "cudaHostAlloc(status word)");
+    g_host_status[*dev] = static_cast<unsigned *>(p);
+    *g_host_status[*dev] = 0;
+  }
+  return THORK_OK;
+}
+
+int thork_status_word(unsigned **d_status) {
+  int dev, rc;
+  if ((rc = status_words(&dev))) return rc;
   *d_status = g_status[dev];
   return THORK_OK;
 }
 
 int thork_host_status_word(unsigned **word) {
   int dev, rc;
-  if ((rc = current_device(&dev))) return rc;
-  std::lock_guard<std::mutex> lk(g_dev_mu);
-  if (!g_host_status[dev]) {
-    void *p = nullptr;
-    // one address for both sides (unified addressing)
-    cudaError_t e = cudaHostAlloc(&p, 16, cudaHostAllocMapped | cudaHostAllocPortable);
-    if (e != cudaSuccess) return thork_cuda_error(e, "cudaHostAlloc(status word)");
-    g_host_status[dev] = static_cast<unsigned *>(p);
-    *g_host_status[dev] = 0;
-  }
+  if ((rc = status_words(&dev))) return rc;
   *word = g_host_status[dev];
   return THORK_OK;
 }
